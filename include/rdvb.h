@@ -542,6 +542,87 @@ int rdvb_pbvrt(const float* rays, int64_t n_rays, const float* transform, float 
                const float* const* biases, const int* layer_flags, int input_relu, void* workspace,
                size_t workspace_bytes, float* out, void* stream);
 
+/* ------------------------------------------ conditioned image blocks ----
+ * Operators of the blocks between an image network's convolutions:
+ * normalisation with an activation, attention of the image's positions to an
+ * encoder's states, and dropout. Beyond the reference, which has none.
+ * RDVB_F32, RDVB_F16 or RDVB_BF16 elements; sums, softmax and statistics in
+ * float32, each result rounded once. No atomics: results repeat bit for bit.
+ */
+
+#define RDVB_ACT_NONE 0
+#define RDVB_ACT_RELU 1
+#define RDVB_ACT_SILU 2 /* z sigmoid(z) */
+#define RDVB_ACT_GELU 3 /* z Phi(z), the error-function form */
+
+/* Group norm with an activation over channels-last maps x [n, rows, c] (rows:
+ * the positions of an image): xhat = (x - mu) rstd with the mean and 1 /
+ * sqrt(variance + eps) of a sample's group (groups divides c; at most 2048)
+ * and y = act(weight_c xhat + bias_c). weight, bias: [c] of param_dtype, or
+ * NULL (1 and 0). stats: [n, groups, 2] fp32 (mean, rstd), or NULL; the
+ * backward pass wants it. workspace: 16-byte aligned,
+ * rdvb_group_norm_workspace_bytes(). n or rows 0: nothing is written.
+ *  _backward: dx of dy, and dweight, dbias [c] fp32 (either may be NULL), the
+ *    sums over samples and rows. */
+int64_t rdvb_group_norm_workspace_bytes(int64_t n, int64_t rows, int c, int groups, int backward);
+int rdvb_group_norm(const void* x, int dtype, int64_t n, int64_t rows, int c, int groups, const void* weight,
+                    const void* bias, int param_dtype, int activation, float eps, void* y, float* stats,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int rdvb_group_norm_backward(const void* dy, const void* x, const float* stats, int dtype, int64_t n, int64_t rows,
+                             int c, int groups, const void* weight, const void* bias, int param_dtype, int activation,
+                             void* dx, float* dweight, float* dbias, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Attention of q [batch, q_len, heads, dim] to k, v [batch, kv_len, kv_heads,
+ * dim] (kv_heads divides heads; dim <= 256): out = softmax(scale q k^T) v over
+ * a sample's allowed keys -- below lengths[sample] (NULL: all; outside [0,
+ * kv_len] it is clamped) and where mask [batch, kv_len] (bytes, mask_stride a
+ * sample; NULL: all) is not 0. A sample without allowed keys gives 0 (lse
+ * -inf, no gradient). What lies at a key that is not allowed is not used,
+ * NaN and infinities included. Strides in elements of (sample, position,
+ * head); the last dimension is dense. */
+typedef struct rdvb_attention {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int32_t* lengths;
+    const uint8_t* mask;
+    int64_t mask_stride;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t q_len;
+    int64_t kv_len;
+    int dtype;
+    int batch;
+    int heads;
+    int kv_heads;
+    int dim;
+    float scale;
+} rdvb_attention;
+
+/* Bytes of the 16-byte aligned workspace that the pass needs (0: may be
+ * NULL), or 0 for a description that the pass refuses. */
+int64_t rdvb_attention_workspace_bytes(const rdvb_attention* a, int backward);
+/* out [batch, q_len, heads, dim] dense; lse [batch, heads, q_len] fp32, the
+ * natural log of the sum of exp(scale q k^T), or NULL. */
+int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                           void* stream);
+/* Gradients of out for dout (both dense, out and lse from the forward pass):
+ * dq as out, dk and dv [batch, kv_len, kv_heads, dim] dense, summed over the
+ * query heads that share a key head; 0 at keys that are not allowed. */
+int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const void* out, const float* lse, void* dq,
+                            void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Dropout: y[i] = residual[i] + (kept ? x[i] / (1 - p) : 0), residual NULL:
+ * 0. Element i is kept iff word i % 4 of the Philox 4x32 block with ten
+ * rounds at counter offset + i / 4 (64 bits, the upper two counter words 0)
+ * and key seed is >= round(p 2^32); no mask is stored, and the same call on
+ * an output gradient (residual NULL) is the backward pass. p in [0, 1 -
+ * 2^-32). y may be x or residual. */
+int rdvb_dropout(const void* x, const void* residual, void* y, int dtype, int64_t n, double p, uint64_t seed,
+                 uint64_t offset, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

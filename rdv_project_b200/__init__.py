@@ -21,6 +21,8 @@ from .conv import (Conv2DTensorOp, Conv2DTensorOpFast, Conv2DTensorOpSimple, Con
 from .rendering import Cameras, VolumeRenderer
 from .volumes import (RaymarchingTransmittance, RatiotrackingTransmittance, TensorGrid, VoxelMajorantField,
                       SphereMajorantField, PBVR, PBVRT, PBVR_NEE, PBVR_ENV, XREnvironmentSampler)
+from .blocks import (group_norm, group_norm_forward, group_norm_backward, cross_attention, cross_attention_forward,
+                     cross_attention_backward, dropout, dropout_backward, GroupNormTensorOp, CrossAttentionTensorOp)
 from ._native import RdvbError, device_status
 
 __all__ = [
@@ -33,5 +35,7 @@ __all__ = [
     "Conv2DTensorOpWindow3x3", "Conv2DTensorOpWinograd3x3", "Conv3x3Winograd", "conv2d_direct",
     "Cameras", "VolumeRenderer", "RaymarchingTransmittance", "RatiotrackingTransmittance", "TensorGrid",
     "VoxelMajorantField", "SphereMajorantField", "PBVR", "PBVRT", "PBVR_NEE", "PBVR_ENV", "XREnvironmentSampler",
+    "group_norm", "group_norm_forward", "group_norm_backward", "cross_attention", "cross_attention_forward",
+    "cross_attention_backward", "dropout", "dropout_backward", "GroupNormTensorOp", "CrossAttentionTensorOp",
     "RdvbError", "device_status",
 ]

@@ -26,6 +26,7 @@ RDVB_ENV_CONSTANT, RDVB_ENV_EQUIRECT = 0, 1
 RDVB_SAMPLER_CLAMP, RDVB_SAMPLER_ALIGNED, RDVB_SAMPLER_LINEAR = 1, 2, 4
 RDVB_PBVRT, RDVB_PBVR_NEE, RDVB_PBVR_ENV = 0, 1, 2
 RDVB_ENCODING_TENSOR_SAMPLER, RDVB_ENCODING_GRID_SAMPLER = 1, 2
+RDVB_ACT_NONE, RDVB_ACT_RELU, RDVB_ACT_SILU, RDVB_ACT_GELU = 0, 1, 2, 3
 RDVB_IPC_HANDLE_BYTES = 64
 RDVB_MAX_PEERS = 7
 
@@ -85,6 +86,15 @@ SIGNATURES = {
     "rdvb_grid_sampler": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_i64, _c_int, _c_int, _c_int, _vp, _vp]),
     "rdvb_pbvr": (_c_int, [_vp, _c_i64, _vp, _vp, _vp, _c_int, _vp, _c_f, _c_int, _c_int, _vp, _vp, _vp, _c_int,
                            _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, ctypes.c_size_t, _vp, _vp]),
+    "rdvb_group_norm_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int, _c_int, _c_int]),
+    "rdvb_group_norm": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_int, _c_int, _vp, _vp, _c_int, _c_int, _c_f, _vp, _vp,
+                                 _vp, ctypes.c_size_t, _vp]),
+    "rdvb_group_norm_backward": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_int, _c_int, _vp, _vp, _c_int,
+                                          _c_int, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "rdvb_attention_workspace_bytes": (_c_i64, [_vp, _c_int]),
+    "rdvb_attention_forward": (_c_int, [_vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "rdvb_attention_backward": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "rdvb_dropout": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _vp]),
 }
 
 
@@ -92,6 +102,14 @@ class Encoding(ctypes.Structure):
     """rdvb_encoding: a sampler of a dense 3-D grid in front of a volume
     node's extinction chain."""
     _fields_ = [("kind", _c_int), ("grid", _vp), ("dims", _c_int * 3), ("features", _c_int), ("flags", _c_int)]
+
+
+class Attention(ctypes.Structure):
+    """rdvb_attention: the inputs of one attention call."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("lengths", _vp), ("mask", _vp), ("mask_stride", _c_i64),
+                ("q_stride", _c_i64 * 3), ("k_stride", _c_i64 * 3), ("v_stride", _c_i64 * 3), ("q_len", _c_i64),
+                ("kv_len", _c_i64), ("dtype", _c_int), ("batch", _c_int), ("heads", _c_int), ("kv_heads", _c_int),
+                ("dim", _c_int), ("scale", _c_f)]
 
 
 class RdvbError(RuntimeError):

@@ -7,6 +7,7 @@ runtime statically so it has no run-time dependency beyond the driver.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -17,10 +18,16 @@ PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "librdvb.so")
-SOURCES = ["rdvb.cu"]
-HEADERS = ["ptx.cuh", "rng.cuh", "mlp_tc.cuh", "mlp_simt.cuh", "winograd.cuh", "winograd_f43.cuh", "raymarch.cuh", "transmittance.cuh",
-           "resample.cuh", "conv_tc.cuh", "sampler.cuh", "pbvr.cuh",
-           "exchange.cuh"]
+OBJ_DIR = os.path.join(LIB_DIR, "obj")
+# source -> the headers it includes (beside include/rdvb.h)
+SOURCES = {
+    "rdvb.cu": ["host.h", "ptx.cuh", "rng.cuh", "mlp_tc.cuh", "mlp_simt.cuh", "winograd.cuh", "winograd_f43.cuh",
+                "raymarch.cuh", "transmittance.cuh", "resample.cuh", "conv_tc.cuh", "sampler.cuh", "pbvr.cuh",
+                "exchange.cuh"],
+    "norm.cu": ["host.h", "types.cuh", "norm.cuh"],
+    "dropout.cu": ["host.h", "types.cuh", "dropout.cuh"],
+    "attention.cu": ["host.h", "types.cuh", "attention.cuh"],
+}
 
 
 def nvcc_path() -> str:
@@ -28,44 +35,67 @@ def nvcc_path() -> str:
     return cand
 
 
-def nvcc_cmd(out: str, extra=()):
+def nvcc_flags():
     return [
-        nvcc_path(),
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-lineinfo", "-O3", "-std=c++17",
         "--expt-relaxed-constexpr",
-        "-Xcompiler", "-fPIC", "-shared",
+        "-Xcompiler", "-fPIC",
         "-I", os.path.join(ROOT, "include"),
         "-I", HERE,
-        "-o", out,
-        *[os.path.join(HERE, s) for s in SOURCES],
-        *extra,
     ]
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _object(source: str) -> str:
+    return os.path.join(OBJ_DIR, os.path.splitext(source)[0] + ".o")
+
+
+def _newer(target: str, deps) -> bool:
+    """Whether target is missing or older than one of deps."""
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(HERE, f) for f in SOURCES + HEADERS] + [os.path.join(ROOT, "include", "rdvb.h")]
+    t = os.path.getmtime(target)
     return any(os.path.exists(d) and os.path.getmtime(d) > t for d in deps)
 
 
-def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) -> str:
-    if not force and not _stale():
-        return LIB_PATH
-    os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = LIB_PATH + ".tmp"
-    extra = ["-Xptxas", "-v"] if ptxas_info else []
-    cmd = nvcc_cmd(tmp, extra)
+def _deps(source: str):
+    return [os.path.join(HERE, f) for f in [source, *SOURCES[source]]] + [os.path.join(ROOT, "include", "rdvb.h")]
+
+
+def _stale() -> bool:
+    return _newer(LIB_PATH, [d for s in SOURCES for d in _deps(s)])
+
+
+def _run(cmd, verbose: bool, what: str) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("nvcc failed building librdvb.so")
-    if verbose or ptxas_info:
+        raise RuntimeError(f"nvcc failed building {what}")
+    if verbose:
         sys.stdout.write(res.stdout + res.stderr)
+
+
+def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) -> str:
+    """Compiles each stale source to an object (in parallel) and links the
+    library; without force, sources whose object is up to date are kept."""
+    if not force and not _stale():
+        return LIB_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    extra = ["-Xptxas", "-v"] if ptxas_info else []
+    todo = [s for s in SOURCES if force or _newer(_object(s), _deps(s))]
+
+    def compile_one(source):
+        tmp = _object(source) + ".tmp"
+        _run([nvcc_path(), *nvcc_flags(), "-c", "-o", tmp, os.path.join(HERE, source), *extra],
+             verbose or ptxas_info, source)
+        os.replace(tmp, _object(source))
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, len(todo))) as pool:
+        list(pool.map(compile_one, todo))
+    tmp = LIB_PATH + ".tmp"
+    _run([nvcc_path(), *nvcc_flags(), "-shared", "-o", tmp, *[_object(s) for s in SOURCES]], verbose, "librdvb.so")
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

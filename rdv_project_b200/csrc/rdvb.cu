@@ -1,6 +1,7 @@
-// C ABI of the rdv B200 hot path (declared in include/rdvb.h). One
-// translation unit: the kernels are included below so that the device status
-// word and the kernels share a module.
+// C ABI of the rdv B200 hot path (declared in include/rdvb.h). The kernels
+// of the path are included below so that the device status word and they
+// share a module; the sources beside this one (host.h) take the word's
+// address as a kernel argument.
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
@@ -15,6 +16,7 @@
 #include <string>
 
 #include "rdvb.h"
+#include "host.h"
 #include "ptx.cuh"
 #include "mlp_tc.cuh"
 #include "mlp_simt.cuh"
@@ -2127,3 +2129,43 @@ int rdvb_mlp_forward_static(const void* x, int x_dtype, int64_t n_rows, int n_la
 }
 
 }  // extern "C"
+
+// ------------------------------------------------- shared with other sources
+namespace rdvb_host {
+
+int fail_text(int code, const char* text) { return ::fail(code, "%s", text); }
+
+int launched(const char* what) { return check_launch(what); }
+
+int device(Device* out) {
+    DeviceInfo* dev = nullptr;
+    if (int rc = current_device(&dev)) return rc;
+    int index = 0;
+    cudaError_t e = cudaGetDevice(&index);
+    if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
+    out->index = index;
+    out->sm_count = dev->sm_count;
+    out->max_smem = dev->max_smem_optin;
+    return RDVB_OK;
+}
+
+int status_word(uint32_t** out) {
+    static uint32_t* at[kMaxDevices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
+    if (dev < 0 || dev >= kMaxDevices) return fail(RDVB_ERR_UNSUPPORTED, "device index %d out of range", dev);
+    std::lock_guard<std::mutex> lock(g_dev_mutex);
+    if (!at[dev]) {
+        void* p = nullptr;
+        e = cudaGetSymbolAddress(&p, rdvb::g_status);
+        if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaGetSymbolAddress: %s", cudaGetErrorString(e));
+        at[dev] = static_cast<uint32_t*>(p);
+    }
+    *out = at[dev];
+    return RDVB_OK;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() { return ::tensor_map_encoder(); }
+
+}  // namespace rdvb_host
