@@ -580,7 +580,9 @@ int rdvb_group_norm_backward(const void* dy, const void* x, const float* stats, 
  * sample; NULL: all) is not 0. A sample without allowed keys gives 0 (lse
  * -inf, no gradient). What lies at a key that is not allowed is not used,
  * NaN and infinities included. Strides in elements of (sample, position,
- * head); the last dimension is dense. */
+ * head); the last dimension is dense. 16-bit inputs whose dim and strides are
+ * multiples of 8 and pointers 16-byte aligned, dim <= 128 and scale >= 0 run
+ * on the tensor cores, others in float32 on CUDA cores. */
 typedef struct rdvb_attention {
     const void* q;
     const void* k;
@@ -604,11 +606,12 @@ typedef struct rdvb_attention {
 /* Bytes of the 16-byte aligned workspace that the pass needs (0: may be
  * NULL), or 0 for a description that the pass refuses. */
 int64_t rdvb_attention_workspace_bytes(const rdvb_attention* a, int backward);
-/* out [batch, q_len, heads, dim] dense; lse [batch, heads, q_len] fp32, the
+/* out [batch, q_len, heads, dim] dense, 16-byte aligned; lse [batch, heads, q_len] fp32, the
  * natural log of the sum of exp(scale q k^T), or NULL. */
 int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void* workspace, size_t workspace_bytes,
                            void* stream);
-/* Gradients of out for dout (both dense, out and lse from the forward pass):
+/* Gradients of out for dout (both dense and 16-byte aligned like the results,
+ * out and lse from the forward pass):
  * dq as out, dk and dv [batch, kv_len, kv_heads, dim] dense, summed over the
  * query heads that share a key head; 0 at keys that are not allowed. */
 int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const void* out, const float* lse, void* dq,

@@ -199,6 +199,12 @@ def _describe(q, k, v, lengths, mask, scale):
     return a, (q, k, v, lengths, mask)
 
 
+def _dense16(t):
+    """t dense and 16-byte aligned, as the kernels read it."""
+    t = _tensor(t).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _cross_attention(q, k, v, lengths, mask, scale, want_lse):
     a, held = _describe(q, k, v, lengths, mask, scale)
     q = held[0]
@@ -226,7 +232,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, lengths=None, mask=None, s
     0 at states that no position attends to."""
     a, held = _describe(q, k, v, lengths, mask, scale)
     q, k = held[0], held[1]
-    dout, out, lse = _tensor(dout).contiguous(), _tensor(out).contiguous(), _tensor(lse).contiguous()
+    dout, out, lse = _dense16(dout), _dense16(out), _tensor(lse).contiguous()
     for name, t in (("dout", dout), ("out", out)):
         _need(t.shape == q.shape and t.dtype == q.dtype, f"{name} must have q's shape and type")
     _need(tuple(lse.shape) == (a.batch, a.heads, a.q_len) and lse.dtype == torch.float32,

@@ -3,7 +3,9 @@
 #include <cmath>
 #include <cstring>
 
+#define RDVB_STATUS_ELSEWHERE
 #include "attention.cuh"
+#include "attention_tc.cuh"
 #include "host.h"
 
 using rdvb_host::aligned;
@@ -38,7 +40,49 @@ int check_pointers(const rdvb_attention* a) {
     return RDVB_OK;
 }
 
-int tile_of(int dim) { return dim > 128 ? 32 : 64; }
+// Whether the tensor-core kernels take the call: 16-bit elements, a head
+// dimension of whole 16-byte pieces up to 128, q, k and v as tensor maps take
+// them (16-byte aligned, strides of whole 16-byte pieces; a sample or head
+// stride of 0 is an axis of one) and a scale that keeps the scores' order.
+bool tensor_core(const rdvb_attention* a) {
+    if (a->dtype == RDVB_F32 || a->dim > 128 || a->dim % 8 || !(a->scale > 0.0f)) return false;
+    if (a->kv_len == 0 || !aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16)) return false;
+    auto fits = [](const int64_t* stride, int64_t batch, int64_t length, int64_t heads) {
+        const int64_t extent[3] = {batch, length, heads};
+        for (int i = 0; i < 3; ++i) {
+            const int64_t s = stride[i];
+            if (extent[i] > 1 && (s % 8 || s < 0 || s >= (1LL << 38) || (s == 0 && i == 1))) return false;
+        }
+        return true;
+    };
+    if (!fits(a->q_stride, a->batch, a->q_len, a->heads) || !fits(a->k_stride, a->batch, a->kv_len, a->kv_heads) ||
+        !fits(a->v_stride, a->batch, a->kv_len, a->kv_heads))
+        return false;
+    return rdvb_host::tensor_map_encoder() != nullptr;
+}
+
+// The map of [batch, length, heads, dim] that a tile of 128 positions of one
+// head is loaded by, in atoms of 64 dimensions; past the ends it reads 0.
+int encode(TcMap* out, const rdvb_attention* a, const void* base, const int64_t* stride, int64_t length, int heads) {
+    out->head_step = heads > 1 && stride[2] != 0;
+    out->batch_step = a->batch > 1 && stride[0] != 0;
+    auto bytes = [](bool walked, int64_t s) -> cuuint64_t { return walked ? s * 2 : 16; };
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a->dim), static_cast<cuuint64_t>(out->head_step ? heads : 1),
+                                static_cast<cuuint64_t>(length),
+                                static_cast<cuuint64_t>(out->batch_step ? a->batch : 1)};
+    const cuuint64_t strides[3] = {bytes(out->head_step, stride[2]), bytes(length > 1, stride[1]),
+                                   bytes(out->batch_step, stride[0])};
+    const cuuint32_t box[4] = {64, 1, kTcTile, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult rc = rdvb_host::tensor_map_encoder()(
+        &out->map, a->dtype == RDVB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+        const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS)
+        return fail(RDVB_ERR_CUDA, "cuTensorMapEncodeTiled returned %d", static_cast<int>(rc));
+    return RDVB_OK;
+}
+
+int tile_of(const rdvb_attention* a, bool tc) { return tc ? kTcTile : a->dim > 128 ? 32 : 64; }
 
 // Parts into which a launch of `tiles` blocks with `items` loop steps each is
 // split: as many as fill the processors about twice, none of fewer than four
@@ -49,30 +93,36 @@ int splits_for(int64_t tiles, int64_t items) {
 }
 
 struct Plan {
-    int forward, dkv;  // splits
-    int64_t forward_len, dkv_len;
-    int64_t forward_bytes, backward_bytes;
-    int64_t delta_bytes, dq_bytes;
+    bool tc;
+    int forward, dq, dkv;  // splits
+    int64_t forward_len, dq_len, dkv_len;
+    int64_t forward_bytes, backward_bytes, delta_bytes;
 };
 
 Plan plan(const rdvb_attention* a) {
     Plan p;
-    const int tile = tile_of(a->dim);
+    p.tc = tensor_core(a);
+    const int tile = tile_of(a, p.tc), back = tile_of(a, false);
     const int64_t q_tiles = ceil_div(a->q_len, tile), k_tiles = ceil_div(a->kv_len, tile);
     const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
     const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
     p.forward = splits_for(q_tiles * a->heads * a->batch, k_tiles);
     p.forward_len = ceil_div(k_tiles, p.forward) * tile;
     p.forward = static_cast<int>(std::max<int64_t>(1, ceil_div(a->kv_len, std::max<int64_t>(p.forward_len, 1))));
-    const int64_t items = q_tiles * (a->heads / a->kv_heads);
-    p.dkv = splits_for(k_tiles * a->kv_heads * a->batch, items);
+    p.forward_bytes = p.forward > 1 ? round16(p.forward * rows * 8) + p.forward * rows * a->dim * 4 : 0;
+    // gradients
+    const int64_t bq_tiles = ceil_div(a->q_len, back), bk_tiles = ceil_div(a->kv_len, back);
+    p.dq = splits_for(bq_tiles * a->heads * a->batch, bk_tiles);
+    p.dq_len = ceil_div(bk_tiles, p.dq) * back;
+    p.dq = static_cast<int>(std::max<int64_t>(1, ceil_div(a->kv_len, std::max<int64_t>(p.dq_len, 1))));
+    const int64_t items = bq_tiles * (a->heads / a->kv_heads);
+    p.dkv = splits_for(bk_tiles * a->kv_heads * a->batch, items);
     p.dkv_len = ceil_div(items, p.dkv);
     p.dkv = static_cast<int>(std::max<int64_t>(1, ceil_div(items, std::max<int64_t>(p.dkv_len, 1))));
-    p.forward_bytes = p.forward > 1 ? round16(p.forward * rows * 8) + p.forward * rows * a->dim * 4 : 0;
     p.delta_bytes = round16(rows * 4);
-    p.dq_bytes = p.forward > 1 ? p.forward * rows * a->dim * 4 : 0;
+    const int64_t dq_bytes = p.dq > 1 ? p.dq * rows * a->dim * 4 : 0;
     const int64_t dkv_bytes = p.dkv > 1 ? 2 * p.dkv * kv_rows * a->dim * 4 : 0;
-    p.backward_bytes = p.delta_bytes + std::max(p.dq_bytes, dkv_bytes);  // the two are joined in turn
+    p.backward_bytes = p.delta_bytes + std::max(dq_bytes, dkv_bytes);  // the two are joined in turn
     return p;
 }
 
@@ -119,6 +169,33 @@ int launch(K kernel, int64_t blocks, int smem, const Params& p, cudaStream_t st,
      : a->dim <= 128 ? launch(kernel<128>, __VA_ARGS__ Shape<128>::bytes, p, st, #kernel)                   \
                      : launch(kernel<256>, __VA_ARGS__ Shape<256>::bytes, p, st, #kernel))
 
+int launch_tc_forward(const rdvb_attention* a, const Params& p, int64_t blocks, cudaStream_t st) {
+    if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "tc_forward_kernel: too many blocks");
+    TcParams t;
+    t.a = p;
+    if (int rc = rdvb_host::status_word(&t.status)) return rc;
+    t.k_steps = static_cast<uint32_t>((a->dim + 15) / 16);
+    t.n_pv = 16 * t.k_steps;
+    t.guarded = a->lengths || a->mask;
+    TcMap q, k, v;
+    if (int rc = encode(&q, a, a->q, a->q_stride, a->q_len, a->heads)) return rc;
+    if (int rc = encode(&k, a, a->k, a->k_stride, a->kv_len, a->kv_heads)) return rc;
+    if (int rc = encode(&v, a, a->v, a->v_stride, a->kv_len, a->kv_heads)) return rc;
+    auto go = [&](auto kernel, uint32_t smem) -> int {
+        cudaError_t e =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        kernel<<<static_cast<unsigned>(blocks), kTcThreads, smem, st>>>(t, q, k, v);
+        return rdvb_host::launched("tc_forward_kernel");
+    };
+    const bool bf16 = a->dtype == RDVB_BF16;
+    if (a->dim <= 64)
+        return bf16 ? go(tc_forward_kernel<64, true>, TcForward<64>::kBytes)
+                    : go(tc_forward_kernel<64, false>, TcForward<64>::kBytes);
+    return bf16 ? go(tc_forward_kernel<128, true>, TcForward<128>::kBytes)
+                : go(tc_forward_kernel<128, false>, TcForward<128>::kBytes);
+}
+
 int simple_launch_check(int64_t blocks, const char* what) {
     return blocks > 0x7fffffffLL ? fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what) : RDVB_OK;
 }
@@ -138,9 +215,8 @@ int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void*
     if (int rc = check(a)) return rc;
     if (a->batch == 0 || a->q_len == 0) return RDVB_OK;
     if (int rc = check_pointers(a)) return rc;
-    const uintptr_t size = a->dtype == RDVB_F32 ? 4 : 2;
-    if (!out || !aligned(out, size) || !aligned(lse, 4))
-        return fail(RDVB_ERR_INVALID_ARG, "out must not be NULL, out and lse aligned to their elements");
+    if (!out || !aligned(out, 16) || !aligned(lse, 4))
+        return fail(RDVB_ERR_INVALID_ARG, "out must be a 16-byte aligned pointer, lse 4-byte aligned");
     const Plan l = plan(a);
     if (l.forward_bytes > 0 && (!workspace || !aligned(workspace, 16) ||
                                 workspace_bytes < static_cast<size_t>(l.forward_bytes)))
@@ -158,8 +234,12 @@ int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void*
     const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
     p.part_stat = static_cast<float*>(workspace);
     p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + round16(p.splits * rows * 8));
-    const int64_t blocks = ceil_div(a->q_len, tile_of(a->dim)) * a->heads * a->batch * p.splits;
-    if (int rc = RDVB_BY_DIM(forward_kernel, kForwardBytes, blocks, )) return rc;
+    const int64_t blocks = ceil_div(a->q_len, tile_of(a, l.tc)) * a->heads * a->batch * p.splits;
+    if (l.tc) {
+        if (int rc = launch_tc_forward(a, p, blocks, st)) return rc;
+    } else if (int rc = RDVB_BY_DIM(forward_kernel, kForwardBytes, blocks, )) {
+        return rc;
+    }
     if (p.splits > 1) {
         const int64_t join = ceil_div(rows, kThreads / 32);
         if (int rc = simple_launch_check(join, "join_forward_kernel")) return rc;
@@ -178,9 +258,9 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
     if ((rows > 0 && (!dq || !dout || !out || !lse)) || (kv_rows > 0 && (!dk || !dv)))
         return fail(RDVB_ERR_INVALID_ARG, "dout, out, lse, dq, dk and dv must not be NULL");
-    if (!aligned(dout, size) || !aligned(out, size) || !aligned(dq, size) || !aligned(dk, size) ||
-        !aligned(dv, size) || !aligned(lse, 4))
-        return fail(RDVB_ERR_INVALID_ARG, "a pointer is not aligned to its element size");
+    if (!aligned(dout, 16) || !aligned(out, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
+        !aligned(lse, 4))
+        return fail(RDVB_ERR_INVALID_ARG, "dout, out, dq, dk and dv must be 16-byte aligned, lse 4-byte aligned");
     if (rows == 0 || kv_rows == 0) {  // no pair: zero gradients
         if (rows == 0 && kv_rows == 0) return RDVB_OK;
         rdvb_host::Device dev;
@@ -201,7 +281,6 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     if (int rc = rdvb_host::device(&dev)) return rc;
     Params p;
     fill(p, a);
-    p.wide = p.wide && aligned(dout, 4 * size) && aligned(out, 4 * size);
     p.out = out;
     p.dout = dout;
     p.lse = const_cast<float*>(lse);
@@ -214,15 +293,15 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     if (int rc = simple_launch_check(delta_blocks, "delta_kernel")) return rc;
     delta_kernel<<<static_cast<unsigned>(delta_blocks), kThreads, 0, st>>>(p);
     if (int rc = rdvb_host::launched("delta_kernel")) return rc;
-    const int tile = tile_of(a->dim);
+    const int tile = tile_of(a, false);
     auto join = [&](const float* part, int splits, int64_t pitch, int64_t n, void* to) -> int {
         const int64_t blocks = ceil_div(n, kThreads);
         if (int rc = simple_launch_check(blocks, "join_kernel")) return rc;
         join_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(part, splits, pitch, n, to, a->dtype);
         return rdvb_host::launched("join_kernel");
     };
-    p.splits = l.forward;
-    p.split_len = l.forward_len;
+    p.splits = l.dq;
+    p.split_len = l.dq_len;
     int64_t blocks = ceil_div(a->q_len, tile) * a->heads * a->batch * p.splits;
     if (int rc = RDVB_BY_DIM(dq_kernel, kBackwardBytes, blocks, )) return rc;
     if (p.splits > 1)

@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
             float m = -INFINITY;
 #pragma unroll
             for (int j = 0; j < kPer; ++j)
-                if (s_ok[tx + 16 * j] != 0.0f) m = fmaxf(m, s[i][j]);
-            m = fmaxf(top[i], half_warp_max(m * c));
+                if (s_ok[tx + 16 * j] != 0.0f) m = fmaxf(m, s[i][j] * c);
+            m = fmaxf(top[i], half_warp_max(m));
             const float base = m == -INFINITY ? 0.0f : m;  // every score so far is -inf
             const float old = exp2f(top[i] - base);
             float sum = 0.0f;

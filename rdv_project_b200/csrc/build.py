@@ -26,7 +26,7 @@ SOURCES = {
                 "exchange.cuh"],
     "norm.cu": ["host.h", "types.cuh", "norm.cuh"],
     "dropout.cu": ["host.h", "types.cuh", "dropout.cuh"],
-    "attention.cu": ["host.h", "types.cuh", "attention.cuh"],
+    "attention.cu": ["host.h", "types.cuh", "ptx.cuh", "attention.cuh", "attention_tc.cuh"],
 }
 
 

@@ -23,9 +23,12 @@ enum : uint32_t {
 };
 
 // Device status word: OR of the kStatus* bits raised by any kernel of this
-// library since the host last cleared it (rdvb_device_status). This library
-// is a single translation unit, so the definition lives here.
+// library since the host last cleared it (rdvb_device_status). It is defined
+// in rdvb.cu's module; kernels of other sources get its address as an
+// argument (RDVB_STATUS_ELSEWHERE).
+#ifndef RDVB_STATUS_ELSEWHERE
 __device__ uint32_t g_status;
+#endif
 
 // A bounded wait gives up after this many nanoseconds (%globaltimer).
 #ifndef RDVB_WAIT_LIMIT_NS
@@ -147,15 +150,18 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 
 // Drain wait used on the abort path: ignores the abort flag, keeps its own
 // time limit.
-__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, uint32_t* status) {
     const uint64_t t0 = global_timer_ns();
     while (!mbar_try_wait_sleep(bar, parity, 500000u)) {
         if (global_timer_ns() - t0 > RDVB_WAIT_LIMIT_NS) {
-            atomicOr(&g_status, kStatusTimeoutDrain);
+            atomicOr(status, kStatusTimeoutDrain);
             return;
         }
     }
 }
+#ifndef RDVB_STATUS_ELSEWHERE
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) { drain_wait(bar, parity, &g_status); }
+#endif
 
 // ------------------------------------------------------- bulk async copies
 // Global -> shared 1-D bulk copy (TMA engine), completion counted on `bar`
