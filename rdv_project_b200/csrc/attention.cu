@@ -6,6 +6,7 @@
 #define RDVB_STATUS_ELSEWHERE
 #include "attention.cuh"
 #include "attention_tc.cuh"
+#include "attention_tc_grad.cuh"
 #include "host.h"
 
 using rdvb_host::aligned;
@@ -96,13 +97,13 @@ struct Plan {
     bool tc;
     int forward, dq, dkv;  // splits
     int64_t forward_len, dq_len, dkv_len;
-    int64_t forward_bytes, backward_bytes, delta_bytes;
+    int64_t forward_bytes, backward_bytes, delta_bytes, q_pad;
 };
 
 Plan plan(const rdvb_attention* a) {
     Plan p;
     p.tc = tensor_core(a);
-    const int tile = tile_of(a, p.tc), back = tile_of(a, false);
+    const int tile = tile_of(a, p.tc), back = tile;
     const int64_t q_tiles = ceil_div(a->q_len, tile), k_tiles = ceil_div(a->kv_len, tile);
     const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
     const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
@@ -119,7 +120,9 @@ Plan plan(const rdvb_attention* a) {
     p.dkv = splits_for(bk_tiles * a->kv_heads * a->batch, items);
     p.dkv_len = ceil_div(items, p.dkv);
     p.dkv = static_cast<int>(std::max<int64_t>(1, ceil_div(items, std::max<int64_t>(p.dkv_len, 1))));
-    p.delta_bytes = round16(rows * 4);
+    p.q_pad = bq_tiles * back;
+    p.delta_bytes = p.tc ? 2 * static_cast<int64_t>(a->batch) * a->heads * p.q_pad * 4 + kPrepBlocks * 8
+                         : round16(rows * 4);
     const int64_t dq_bytes = p.dq > 1 ? p.dq * rows * a->dim * 4 : 0;
     const int64_t dkv_bytes = p.dkv > 1 ? 2 * p.dkv * kv_rows * a->dim * 4 : 0;
     p.backward_bytes = p.delta_bytes + std::max(dq_bytes, dkv_bytes);  // the two are joined in turn
@@ -194,6 +197,70 @@ int launch_tc_forward(const rdvb_attention* a, const Params& p, int64_t blocks, 
                     : go(tc_forward_kernel<64, false>, TcForward<64>::kBytes);
     return bf16 ? go(tc_forward_kernel<128, true>, TcForward<128>::kBytes)
                 : go(tc_forward_kernel<128, false>, TcForward<128>::kBytes);
+}
+
+// dQ, dK and dV of a call that tensor_core() takes; `join` sums parts.
+template <typename Join>
+int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* workspace, cudaStream_t st, Join join) {
+    GradParams g;
+    if (int rc = rdvb_host::status_word(&g.status)) return rc;
+    const int64_t stats = static_cast<int64_t>(a->batch) * a->heads * l.q_pad;
+    g.neg_lse = static_cast<float*>(workspace);
+    g.neg_delta = g.neg_lse + stats;
+    g.norms = reinterpret_cast<float2*>(g.neg_delta + stats);
+    g.q_pad = l.q_pad;
+    g.k_steps = static_cast<uint32_t>((a->dim + 15) / 16);
+    g.n_pv = 16 * g.k_steps;
+    g.guarded = a->lengths || a->mask;
+    TcMap q, k, v, d;
+    const int64_t dense[3] = {a->q_len * a->heads * a->dim, static_cast<int64_t>(a->heads) * a->dim, a->dim};
+    if (int rc = encode(&q, a, a->q, a->q_stride, a->q_len, a->heads)) return rc;
+    if (int rc = encode(&k, a, a->k, a->k_stride, a->kv_len, a->kv_heads)) return rc;
+    if (int rc = encode(&v, a, a->v, a->v_stride, a->kv_len, a->kv_heads)) return rc;
+    if (int rc = encode(&d, a, p.dout, dense, a->q_len, a->heads)) return rc;
+    const bool bf16 = a->dtype == RDVB_BF16, narrow = a->dim <= 64;
+    g.a = p;
+    if (narrow)
+        bf16 ? tc_prep_kernel<8, true><<<kPrepBlocks, kThreads, 0, st>>>(g)
+             : tc_prep_kernel<8, false><<<kPrepBlocks, kThreads, 0, st>>>(g);
+    else
+        bf16 ? tc_prep_kernel<16, true><<<kPrepBlocks, kThreads, 0, st>>>(g)
+             : tc_prep_kernel<16, false><<<kPrepBlocks, kThreads, 0, st>>>(g);
+    if (int rc = rdvb_host::launched("tc_prep_kernel")) return rc;
+    auto go = [&](auto kernel, uint32_t smem, int64_t blocks, const char* what) -> int {
+        if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what);
+        cudaError_t e =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        kernel<<<static_cast<unsigned>(blocks), kGradThreads, smem, st>>>(g, q, k, v, d);
+        return rdvb_host::launched(what);
+    };
+    const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
+    const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
+    g.a.splits = l.dq;
+    g.a.split_len = l.dq_len;
+    int64_t blocks = l.q_pad / kTcTile * a->heads * a->batch * l.dq;
+    if (int rc = narrow ? (bf16 ? go(tc_dq_kernel<64, true>, TcDq<64>::kBytes, blocks, "tc_dq_kernel")
+                                : go(tc_dq_kernel<64, false>, TcDq<64>::kBytes, blocks, "tc_dq_kernel"))
+                        : (bf16 ? go(tc_dq_kernel<128, true>, TcDq<128>::kBytes, blocks, "tc_dq_kernel")
+                                : go(tc_dq_kernel<128, false>, TcDq<128>::kBytes, blocks, "tc_dq_kernel")))
+        return rc;
+    if (l.dq > 1)
+        if (int rc = join(p.part, l.dq, rows * a->dim, rows * a->dim, p.dq)) return rc;
+    g.a.splits = l.dkv;
+    g.a.split_len = l.dkv_len;
+    blocks = ceil_div(a->kv_len, kTcTile) * a->kv_heads * a->batch * l.dkv;
+    if (int rc = narrow ? (bf16 ? go(tc_dkv_kernel<64, true>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel")
+                                : go(tc_dkv_kernel<64, false>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel"))
+                        : (bf16 ? go(tc_dkv_kernel<128, true>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel")
+                                : go(tc_dkv_kernel<128, false>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel")))
+        return rc;
+    if (l.dkv > 1) {
+        const int64_t n = kv_rows * a->dim;
+        if (int rc = join(p.part, l.dkv, 2 * n, n, p.dk)) return rc;
+        if (int rc = join(p.part + n, l.dkv, 2 * n, n, p.dv)) return rc;
+    }
+    return RDVB_OK;
 }
 
 int simple_launch_check(int64_t blocks, const char* what) {
@@ -289,17 +356,18 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     p.dq = dq;
     p.dk = dk;
     p.dv = dv;
-    const int64_t delta_blocks = ceil_div(rows, kThreads / 32);
-    if (int rc = simple_launch_check(delta_blocks, "delta_kernel")) return rc;
-    delta_kernel<<<static_cast<unsigned>(delta_blocks), kThreads, 0, st>>>(p);
-    if (int rc = rdvb_host::launched("delta_kernel")) return rc;
-    const int tile = tile_of(a, false);
     auto join = [&](const float* part, int splits, int64_t pitch, int64_t n, void* to) -> int {
         const int64_t blocks = ceil_div(n, kThreads);
         if (int rc = simple_launch_check(blocks, "join_kernel")) return rc;
         join_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(part, splits, pitch, n, to, a->dtype);
         return rdvb_host::launched("join_kernel");
     };
+    if (l.tc) return launch_tc_backward(a, l, p, workspace, st, join);
+    const int64_t delta_blocks = ceil_div(rows, kThreads / 32);
+    if (int rc = simple_launch_check(delta_blocks, "delta_kernel")) return rc;
+    delta_kernel<<<static_cast<unsigned>(delta_blocks), kThreads, 0, st>>>(p);
+    if (int rc = rdvb_host::launched("delta_kernel")) return rc;
+    const int tile = tile_of(a, false);
     p.splits = l.dq;
     p.split_len = l.dq_len;
     int64_t blocks = ceil_div(a->q_len, tile) * a->heads * a->batch * p.splits;

@@ -30,8 +30,8 @@ namespace attn {
 constexpr int kTcTile = 128;       // query rows and keys of a tile
 constexpr int kTcThreads = 8 * 32;  // one warp is idle: registers are shared out by groups of four
 // Registers of a thread at launch (two blocks fill a processor's 65,536), and
-// after the softmax warps have taken some of the others' (192 + 64 = 2 x 128).
-constexpr int kTcRegisters = 128, kSoftmaxRegisters = 192, kOtherRegisters = 64;
+// after the softmax warps have taken some of the others' (208 + 48 = 2 x 128).
+constexpr int kTcRegisters = 128, kSoftmaxRegisters = 208, kOtherRegisters = 48;
 constexpr float kGrowth = 8.0f;    // log2 of the growth of a row's maximum that O is rescaled at
 
 struct TcParams {
@@ -359,12 +359,12 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             any |= !bits.none();
             if (!(ok = mbar_wait_warp(s_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
             tc_fence_after();
-            uint32_t r[4][32];
+            uint32_t r[8][16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_ld32(row_base + F::kColS + 32 * j, r[j]);
-            tmem_wait_ld32(r[0]);
+            for (int j = 0; j < 8; ++j) tmem_ld16(row_base + F::kColS + 16 * j, r[j]);
+            tmem_wait_ld(r[0]);
 #pragma unroll
-            for (int j = 1; j < 4; ++j) reg_barrier32(r[j]);
+            for (int j = 1; j < 8; ++j) reg_barrier(r[j]);
             if (F::kOwnP) {  // S has been read
                 tc_fence_before();
                 __syncwarp();
@@ -372,16 +372,17 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             }
             if (!whole) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) r[j][e] = bits.w[j] >> e & 1u ? r[j][e] : 0xff800000u;
+                    for (int e = 0; e < 16; ++e)
+                        r[j][e] = bits.w[j / 2] >> (j % 2 * 16 + e) & 1u ? r[j][e] : 0xff800000u;
             }
             float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int e = 0; e < 32; e += 2)
-                    high[j] = fmaxf(fmaxf(high[j], __uint_as_float(r[j][e])), __uint_as_float(r[j][e + 1]));
+                for (int e = 0; e < 16; e += 2)
+                    high[j & 3] = fmaxf(fmaxf(high[j & 3], __uint_as_float(r[j][e])), __uint_as_float(r[j][e + 1]));
             const float m = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * c;
             const bool grows = m > top + kGrowth || (top == -INFINITY && m > -INFINITY);
             if (i > 0 && !mbar_wait_warp(o_full, (i - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull)) {
@@ -409,10 +410,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             const float minus = top == -INFINITY ? 0.0f : -top;
             float sum[4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t packed[16];
+            for (int j = 0; j < 8; ++j) {
+                uint32_t packed[8];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
+                for (int e = 0; e < 16; e += 2) {
                     float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
                     fma_f32x2(x, y, c, minus);
                     x = exp2_approx(x);
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                     add_f32x2(sum[e & 2], sum[(e & 2) + 1], x, y);
                     packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
                 }
-                tmem_st16(row_base + F::kColP + 16 * j, packed);
+                tmem_st8(row_base + F::kColP + 8 * j, packed);
             }
             total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
@@ -480,6 +481,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         }
     }
     tc_fence_before();
+    __syncwarp();
     __syncthreads();
     if (warp == 5) {
         tmem_relinquish();

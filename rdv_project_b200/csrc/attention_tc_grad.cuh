@@ -1,0 +1,686 @@
+// Gradients of attention on the tensor cores (attention.cuh has the
+// mathematics, attention_tc.cuh the tile formats and the conditions).
+//
+// Two kernels recompute S and dP = dO V^T, so that dQ, dK and dV each have
+// one owner and a fixed order of summation: seven products a pair of tiles
+// instead of the five of one kernel that adds dQ up in memory, and no
+// atomics. One block a processor, 512 TMEM columns. Warps 0-7: probabilities
+// and score gradients, a thread a row (a lane of TMEM) and half the columns.
+// Warp 8: loads. Warp 9: products. Warp 10: zeroes rows of K whose keys are
+// not allowed (dQ).
+//
+// P and dS are rounded to the inputs' type, as the tensor cores take them.
+// float16 has few exponents: P is held times 2^15 (P <= 1), dS times 2^E with
+// the largest E that keeps 2 max|dO| max|V| 2^E <= 2^15, a bound of |dS|, so
+// that gradients keep their digits whatever the loss was scaled by.
+#pragma once
+#include <cstdint>
+
+#include "attention_tc.cuh"
+
+namespace rdvb {
+namespace attn {
+
+constexpr int kGradThreads = 12 * 32;
+constexpr int kPrepBlocks = 296;
+
+struct GradParams {
+    Params a;
+    uint32_t* status;
+    float* neg_lse;    // [batch, heads, q_pad]: -lse log2 e; -inf past q_len
+    float* neg_delta;  // [batch, heads, q_pad]: -rowsum(dO O); 0 past q_len
+    float2* norms;     // [kPrepBlocks]: largest |dO|^2 and |V|^2 of a row (float16)
+    int64_t q_pad;     // q_len rounded up to whole tiles
+    uint32_t k_steps, n_pv;
+    int guarded;
+};
+
+// neg_lse, neg_delta and norms: kLanes lanes a row, 16 bytes each.
+template <int kLanes, bool kBf16>
+__global__ void __launch_bounds__(kThreads) tc_prep_kernel(const GradParams p) {
+    const Params& a = p.a;
+    const int sub = threadIdx.x % kLanes;
+    const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / kLanes;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kLanes);
+    auto load8 = [&](const void* src, int64_t at, float (&v)[8]) {
+        if (kBf16)
+            load_f32<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16*>(src) + at, v);
+        else
+            load_f32<__half, 8>(static_cast<const __half*>(src) + at, v);
+    };
+    const bool in = sub * 8 < a.dim;
+    const int64_t rows = static_cast<int64_t>(a.batch) * p.q_pad * a.heads;
+    const int64_t rounds = (rows + step - 1) / step;  // the same for every lane of a warp
+    float most_do = 0.0f, most_v = 0.0f;
+    for (int64_t i = 0; i < rounds; ++i) {
+        const int64_t row = first + i * step;
+        const int64_t h = row % a.heads, q = row / a.heads % p.q_pad, b = row / a.heads / p.q_pad;
+        const bool real = row < rows && q < a.q_len;
+        float dot = 0.0f, norm = 0.0f;
+        if (real && in) {
+            const int64_t at = ((b * a.q_len + q) * a.heads + h) * a.dim + sub * 8;
+            float o[8], g[8];
+            load8(a.out, at, o);
+            load8(a.dout, at, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                dot = fmaf(o[j], g[j], dot);
+                norm = fmaf(g[j], g[j], norm);
+            }
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) {
+            dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (!kBf16) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+        }
+        if (row < rows && sub == 0) {
+            const int64_t at = (b * a.heads + h) * p.q_pad + q;
+            p.neg_delta[at] = real ? -dot : 0.0f;
+            p.neg_lse[at] = real ? -a.lse[(b * a.heads + h) * a.q_len + q] * kLog2e : -INFINITY;
+        }
+        if (!kBf16) most_do = fmaxf(most_do, norm);
+    }
+    if (kBf16) return;
+    const int64_t v_rows = static_cast<int64_t>(a.batch) * a.kv_len * a.kv_heads;
+    const int64_t v_rounds = (v_rows + step - 1) / step;
+    for (int64_t i = 0; i < v_rounds; ++i) {
+        const int64_t row = first + i * step;
+        const int64_t h = row % a.kv_heads, key = row / a.kv_heads % a.kv_len, b = row / a.kv_heads / a.kv_len;
+        float norm = 0.0f;
+        if (row < v_rows && in && allowed(a, static_cast<int>(b), key, length_of(a, static_cast<int>(b)))) {
+            float v[8];
+            load8(a.v, b * a.vs.batch + key * a.vs.pos + h * a.vs.head + sub * 8, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) norm = fmaf(v[j], v[j], norm);
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+        most_v = fmaxf(most_v, norm);
+    }
+    __shared__ float s_most[2][kThreads / 32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        most_do = fmaxf(most_do, __shfl_xor_sync(0xffffffffu, most_do, o));
+        most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, o));
+    }
+    if (threadIdx.x % 32 == 0) {
+        s_most[0][threadIdx.x / 32] = most_do;
+        s_most[1][threadIdx.x / 32] = most_v;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kThreads / 32; ++i) {
+            most_do = fmaxf(most_do, s_most[0][i]);
+            most_v = fmaxf(most_v, s_most[1][i]);
+        }
+        p.norms[blockIdx.x] = make_float2(most_do, most_v);
+    }
+}
+
+// E of dS's factor 2^E; 0 for bfloat16. The same in every thread of a warp.
+template <bool kBf16>
+__device__ __forceinline__ float grad_exponent(const GradParams& p) {
+    if (kBf16) return 0.0f;
+    float x = 0.0f, y = 0.0f;
+    for (int i = threadIdx.x & 31; i < kPrepBlocks; i += 32) {
+        const float2 n = p.norms[i];
+        x = fmaxf(x, n.x);
+        y = fmaxf(y, n.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+    }
+    const float bound = 2.0f * sqrtf(x) * sqrtf(y);
+    if (!(bound > 0.0f && bound < INFINITY)) return 0.0f;
+    return fminf(fmaxf(floorf(15.0f - log2f(bound)), -100.0f), 100.0f);
+}
+
+// (a0, a1) * (b0, b1) in one packed instruction.
+__device__ __forceinline__ void mul_f32x2(float& a0, float& a1, float b0, float b1) {
+    uint64_t pa, pb, pd;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b0), "f"(b1));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(pd) : "l"(pa), "l"(pb));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
+}
+// (a0 b + c0, a1 b + c1) in one packed instruction.
+__device__ __forceinline__ void fma_f32x2(float& a0, float& a1, float b, float c0, float c1) {
+    uint64_t pa, pb, pc, pd;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(pb) : "f"(b));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pc) : "f"(c0), "f"(c1));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(pd) : "l"(pa), "l"(pb), "l"(pc));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
+}
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// D += A B^T with both operands K-major tiles of 128 rows (S, dP), fresh.
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t steps, uint32_t idesc) {
+    for (uint32_t j = 0; j < steps; ++j) {
+        const uint32_t at = (j >> 2) * (kTcTile * 128) + (j & 3) * 32;
+        umma_f16(d, umma_desc_sw128(a + at), umma_desc_sw128(b + at), idesc, j > 0);
+    }
+}
+// D += A B with A in TMEM in two halves 64 columns apart (P, dS), B a tile
+// of 128 rows taken along them.
+__device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+    for (uint32_t j = 0; j < kTcTile / 16; ++j)
+        umma_f16_ts(d, a + (j >> 2) * 64 + (j & 3) * 8, umma_desc_mn_sw128(b + j * 2048, kTcTile * 128), idesc,
+                    !first || j > 0);
+}
+
+// Stores 16 columns of a gradient row from accumulators: 16-bit, or float32
+// parts.
+template <bool kBf16>
+__device__ __forceinline__ void store_columns(const Params& a, void* out, float* part, int64_t at, int d,
+                                              const uint32_t (&r)[16], float f, bool on) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 8) {
+        if (d + e >= a.dim) return;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = on ? __uint_as_float(r[e + k]) * f : 0.0f;
+        if (part) {
+            *reinterpret_cast<float4*>(part + at + d + e) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(part + at + d + e + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = kBf16 ? pack_bf16x2(v[2 * k], v[2 * k + 1]) : pack_f16x2(v[2 * k], v[2 * k + 1]);
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at + d + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------ dQ
+//
+// A block: 128 query rows of one head over the keys of one split. The
+// products run in the order dQ(i), dP(i + 1), S(i + 2): S has two buffers
+// (dS(i) replaces S(i)), dP one.
+template <int DP>
+struct TcDq {
+    static constexpr int kAtoms = DP / 64, kKStages = 3, kVStages = 2;
+    static constexpr uint32_t kTileBytes = kTcTile * DP * 2;
+    static constexpr uint32_t kOffDo = kTileBytes, kOffK = 2 * kTileBytes, kOffV = kOffK + kKStages * kTileBytes,
+                              kOffBar = kOffV + kVStages * kTileBytes;
+    static constexpr uint32_t kBytes = kOffBar + 256 + 1024;
+    static constexpr uint32_t kColS = 0, kColDp = 256, kColDq = 384;
+};
+
+template <int DP, bool kBf16>
+__global__ void __launch_bounds__(kGradThreads, 1)
+    tc_dq_kernel(const GradParams p, const __grid_constant__ TcMap map_q, const __grid_constant__ TcMap map_k,
+                 const __grid_constant__ TcMap map_v, const __grid_constant__ TcMap map_do) {
+    using F = TcDq<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t s_q = base, s_do = base + F::kOffDo, s_k = base + F::kOffK, s_v = base + F::kOffV,
+                   bars = base + F::kOffBar;
+    const uint32_t q_full = bars, dp_full = bars + 8, ds_full = bars + 16, dq_done = bars + 24, drain = bars + 32,
+                   s_full = bars + 40, k_tma = bars + 56, k_ok = bars + 80, k_empty = bars + 104,
+                   v_full = bars + 128, v_empty = bars + 144;
+    const uint32_t tmem_slot = bars + 160;
+    volatile uint32_t* abort_flag =
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 164);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Params& a = p.a;
+    const TcPlace t = tc_place(a);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0u;
+        mbar_init(q_full, 2);  // Q and dO
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        mbar_init(dq_done, 1);
+        mbar_init(drain, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(v_full + 8 * i, 1);
+            mbar_init(v_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < F::kKStages; ++i) {
+            mbar_init(k_tma + 8 * i, 1);
+            mbar_init(k_ok + 8 * i, 1);
+            mbar_init(k_empty + 8 * i, 1);
+        }
+        fence_mbarrier_init();
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+    if (warp == 8) {
+        if (lane == 0 && t.tiles > 0) {
+            int k_sent = 0, v_sent = 0;
+            tc_load<F::kAtoms>(s_q, map_q, t.h, t.q0, t.b, q_full);
+            tc_load<F::kAtoms>(s_do, map_do, t.h, t.q0, t.b, q_full);
+            for (int i = 0; i < t.tiles; ++i) {
+                const int sk = i % F::kKStages, sv = i % F::kVStages;
+                const int64_t k0 = t.begin + static_cast<int64_t>(i) * kTcTile;
+                if (!mbar_wait(k_empty + 8 * sk, ((i / F::kKStages) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutXEmpty))
+                    break;
+                tc_load<F::kAtoms>(s_k + sk * F::kTileBytes, map_k, t.hk, k0, t.b, k_tma + 8 * sk);
+                ++k_sent;
+                if (!mbar_wait(v_empty + 8 * sv, ((i / F::kVStages) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutXEmpty))
+                    break;
+                tc_load<F::kAtoms>(s_v + sv * F::kTileBytes, map_v, t.hk, k0, t.b, v_full + 8 * sv);
+                ++v_sent;
+            }
+            drain_wait(q_full, 0, p.status);
+            for (int s = 0; s < F::kKStages; ++s)
+                if (k_sent > s) drain_wait(k_tma + 8 * s, ((k_sent - 1 - s) / F::kKStages) & 1, p.status);
+            for (int s = 0; s < F::kVStages; ++s)
+                if (v_sent > s) drain_wait(v_full + 8 * s, ((v_sent - 1 - s) / F::kVStages) & 1, p.status);
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && t.tiles > 0) {
+            const uint32_t idesc = umma_idesc_f16(kTcTile, kBf16);
+            const uint32_t idesc_q = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
+            const uint32_t k_ready = p.guarded ? k_ok : k_tma;
+            auto score = [&](int i) {
+                const int s = i % F::kKStages;
+                if (!mbar_wait(k_ready + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                    return false;
+                tc_fence_after();
+                product_rows(tmem + F::kColS + (i & 1) * 128, s_q, s_k + s * F::kTileBytes, p.k_steps, idesc);
+                umma_commit(s_full + 8 * (i & 1));
+                return true;
+            };
+            auto reach = [&](int i) {  // dP(i)
+                const int s = i % F::kVStages;
+                if (!mbar_wait(v_full + 8 * s, (i / F::kVStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                    return false;
+                tc_fence_after();
+                product_rows(tmem + F::kColDp, s_do, s_v + s * F::kTileBytes, p.k_steps, idesc);
+                umma_commit(v_empty + 8 * s);
+                umma_commit(dp_full);
+                return true;
+            };
+            bool ok = mbar_wait(q_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0) && reach(0);
+            if (t.tiles > 1) ok = ok && score(1);
+            for (int i = 0; ok && i < t.tiles; ++i) {
+                const int s = i % F::kKStages;
+                ok = mbar_wait(ds_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull);
+                if (!ok) break;
+                tc_fence_after();
+                product_columns(tmem + F::kColDq, tmem + F::kColS + (i & 1) * 128, s_k + s * F::kTileBytes, idesc_q,
+                                i == 0);
+                umma_commit(k_empty + 8 * s);
+                umma_commit(dq_done);
+                if (i + 1 < t.tiles) ok = reach(i + 1);  // dP(i) was read before ds_full
+                if (ok && i + 2 < t.tiles)
+                    ok = mbar_wait(dq_done, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && score(i + 2);
+            }
+            umma_commit(drain);
+            drain_wait(drain, 0, p.status);
+        }
+    } else if (warp == 10) {
+        if (p.guarded) {
+            for (int i = 0; i < t.tiles; ++i) {
+                const int s = i % F::kKStages;
+                const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+                if (!mbar_wait_warp(k_tma + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                    break;
+                if (!bits.all()) {
+                    zero_rows<F::kAtoms>(s_k + s * F::kTileBytes, bits);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(k_ok + 8 * s);
+            }
+        }
+    } else if (warp < 8) {
+        const int half = warp >> 2;
+        const uint32_t row_base = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+        const int64_t q = t.q0 + (warp & 3) * 32 + lane;
+        const float c = a.scale * kLog2e;
+        const float e2 = grad_exponent<kBf16>(p);
+        const int64_t stat = (static_cast<int64_t>(t.b) * a.heads + t.h) * p.q_pad + q;
+        const float minus = p.neg_lse[stat] + e2, neg_delta = p.neg_delta[stat];
+        bool ok = true, any = false;
+        for (int i = 0; i < t.tiles; ++i) {
+            const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+            const bool whole = bits.all();
+            any |= !bits.none();
+            const uint32_t s_col = row_base + F::kColS + (i & 1) * 128 + half * 64;
+            if (!(ok = mbar_wait_warp(s_full + 8 * (i & 1), (i >> 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull)))
+                break;
+            tc_fence_after();
+            uint32_t r[2][32];
+            tmem_ld32(s_col, r[0]);
+            tmem_ld32(s_col + 32, r[1]);
+            tmem_wait_ld32(r[0]);
+            reg_barrier32(r[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
+                    fma_f32x2(x, y, c, minus);
+                    r[j][e] = __float_as_uint(exp2_approx(x));
+                    r[j][e + 1] = __float_as_uint(exp2_approx(y));
+                }
+            if (!(ok = mbar_wait_warp(dp_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t d[32], packed[16];
+                tmem_ld32(row_base + F::kColDp + half * 64 + 32 * j, d);
+                tmem_wait_ld32(d);
+                const uint32_t word = half ? bits.w[2 + j] : bits.w[j];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x = __uint_as_float(d[e]), y = __uint_as_float(d[e + 1]);
+                    add_f32x2(x, y, neg_delta, neg_delta);
+                    mul_f32x2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
+                    if (!whole) {
+                        x = word >> e & 1u ? x : 0.0f;
+                        y = word >> (e + 1) & 1u ? y : 0.0f;
+                    }
+                    packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                }
+                tmem_st16(s_col + 16 * j, packed);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_full);
+        }
+        if (t.tiles > 0 && ok) ok = mbar_wait_warp(drain, 0, abort_flag, p.status, kStatusTimeoutAccFull);
+        tc_fence_after();
+        const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;
+        const int64_t row = (t.b * a.q_len + q) * a.heads + t.h;
+        float* part = a.splits > 1 ? a.part + t.split * rows * a.dim : nullptr;
+        const float f = a.scale * exp2f(-e2);
+#pragma unroll 1
+        for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 16) {
+            if (d >= a.dim) break;
+            uint32_t r[16] = {};
+            if (t.tiles > 0) {
+                tmem_ld16(row_base + F::kColDq + d, r);
+                tmem_wait_ld(r);
+            }
+            if (ok && q < a.q_len) store_columns<kBf16>(a, a.dq, part, row * a.dim, d, r, f, any);
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (warp == 9) {
+        tmem_relinquish();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------- dK, dV
+//
+// A block: 128 keys of one key head over the (query head, query tile) pairs
+// of one split, with keys as TMEM lanes: S^T = K Q^T, dP^T = V dO^T, P^T and
+// dS^T replace them, dV += P^T dO, dK += dS^T Q. The products run in the
+// order dV(i), dK(i), S(i + 1), dP(i + 1); the exponentials of i + 1 run while
+// dP(i + 1) does, dS(i) while dV(i) does.
+template <int DP>
+struct TcDkv {
+    static constexpr int kAtoms = DP / 64, kStages = 2;
+    static constexpr uint32_t kTileBytes = kTcTile * DP * 2;
+    static constexpr uint32_t kOffV = kTileBytes, kOffQ = 2 * kTileBytes, kOffDo = kOffQ + kStages * kTileBytes,
+                              kOffStat = kOffDo + kStages * kTileBytes;  // [stage][-lse, -delta][128]
+    static constexpr uint32_t kOffBar = kOffStat + kStages * 1024;
+    static constexpr uint32_t kBytes = kOffBar + 256 + 1024;
+    static constexpr uint32_t kColS = 0, kColDp = 128, kColDv = 256, kColDk = 384;
+};
+
+template <int DP, bool kBf16>
+__global__ void __launch_bounds__(kGradThreads, 1)
+    tc_dkv_kernel(const GradParams p, const __grid_constant__ TcMap map_q, const __grid_constant__ TcMap map_k,
+                  const __grid_constant__ TcMap map_v, const __grid_constant__ TcMap map_do) {
+    using F = TcDkv<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t s_k = base, s_v = base + F::kOffV, s_q = base + F::kOffQ, s_do = base + F::kOffDo,
+                   s_stat = base + F::kOffStat, bars = base + F::kOffBar;
+    const uint32_t kv_full = bars, s_full = bars + 8, p_full = bars + 16, dp_full = bars + 24, ds_full = bars + 32,
+                   dv_done = bars + 40, dk_done = bars + 48, drain = bars + 56, q_full = bars + 64,
+                   q_empty = bars + 80, do_full = bars + 96, do_empty = bars + 112;
+    const uint32_t tmem_slot = bars + 128;
+    volatile uint32_t* abort_flag =
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 132);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Params& a = p.a;
+    const uint32_t k_tiles = static_cast<uint32_t>((a.kv_len + kTcTile - 1) / kTcTile);
+    const int q_tiles = static_cast<int>(p.q_pad / kTcTile);
+    uint32_t id = blockIdx.x;
+    const int64_t k0 = static_cast<int64_t>(id % k_tiles) * kTcTile;
+    id /= k_tiles;
+    const int hk = id % a.kv_heads;
+    id /= a.kv_heads;
+    const int b = id % a.batch, split = id / a.batch;
+    const KeyBits bits = key_bits(a, b, k0, length_of(a, b));
+    const int first = static_cast<int>(split * a.split_len);
+    const int last = min(q_tiles * a.group, static_cast<int>(first + a.split_len));
+    const int items = bits.none() ? 0 : last - first;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0u;
+        mbar_init(kv_full, 2);
+        mbar_init(s_full, 1);
+        mbar_init(p_full, 8);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        mbar_init(dv_done, 1);
+        mbar_init(dk_done, 1);
+        mbar_init(drain, 1);
+        for (int i = 0; i < F::kStages; ++i) {
+            mbar_init(q_full + 8 * i, 2);  // the tile and its -lse
+            mbar_init(q_empty + 8 * i, 1);
+            mbar_init(do_full + 8 * i, 2);  // the tile and its -delta
+            mbar_init(do_empty + 8 * i, 1);
+        }
+        fence_mbarrier_init();
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+    if (warp == 8) {
+        if (lane == 0 && items > 0) {
+            int q_sent = 0, do_sent = 0;
+            tc_load<F::kAtoms>(s_k, map_k, hk, k0, b, kv_full);
+            tc_load<F::kAtoms>(s_v, map_v, hk, k0, b, kv_full);
+            for (int i = 0; i < items; ++i) {
+                const int s = i % F::kStages;
+                const uint32_t parity = ((i / F::kStages) & 1) ^ 1;
+                const int h = hk * a.group + (first + i) / q_tiles;
+                const int64_t q0 = static_cast<int64_t>((first + i) % q_tiles) * kTcTile;
+                const int64_t stat = (static_cast<int64_t>(b) * a.heads + h) * p.q_pad + q0;
+                if (!mbar_wait(q_empty + 8 * s, parity, abort_flag, p.status, kStatusTimeoutXEmpty)) break;
+                tc_load<F::kAtoms>(s_q + s * F::kTileBytes, map_q, h, q0, b, q_full + 8 * s);
+                mbar_arrive_expect_tx(q_full + 8 * s, 512);
+                bulk_g2s(s_stat + s * 1024, p.neg_lse + stat, 512, q_full + 8 * s);
+                ++q_sent;
+                if (!mbar_wait(do_empty + 8 * s, parity, abort_flag, p.status, kStatusTimeoutXEmpty)) break;
+                tc_load<F::kAtoms>(s_do + s * F::kTileBytes, map_do, h, q0, b, do_full + 8 * s);
+                mbar_arrive_expect_tx(do_full + 8 * s, 512);
+                bulk_g2s(s_stat + s * 1024 + 512, p.neg_delta + stat, 512, do_full + 8 * s);
+                ++do_sent;
+            }
+            drain_wait(kv_full, 0, p.status);
+            for (int s = 0; s < F::kStages; ++s) {
+                if (q_sent > s) drain_wait(q_full + 8 * s, ((q_sent - 1 - s) / F::kStages) & 1, p.status);
+                if (do_sent > s) drain_wait(do_full + 8 * s, ((do_sent - 1 - s) / F::kStages) & 1, p.status);
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && items > 0) {
+            const uint32_t idesc = umma_idesc_f16(kTcTile, kBf16);
+            const uint32_t idesc_d = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
+            auto score = [&](int i) {
+                const int s = i % F::kStages;
+                if (!mbar_wait(q_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                    return false;
+                tc_fence_after();
+                product_rows(tmem + F::kColS, s_k, s_q + s * F::kTileBytes, p.k_steps, idesc);
+                umma_commit(s_full);
+                return true;
+            };
+            auto reach = [&](int i) {
+                const int s = i % F::kStages;
+                if (!mbar_wait(do_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                    return false;
+                tc_fence_after();
+                product_rows(tmem + F::kColDp, s_v, s_do + s * F::kTileBytes, p.k_steps, idesc);
+                umma_commit(dp_full);
+                return true;
+            };
+            bool ok = mbar_wait(kv_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0) && reach(0);
+            for (int i = 0; ok && i < items; ++i) {
+                const int s = i % F::kStages;
+                if (!(ok = mbar_wait(p_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull))) break;
+                tc_fence_after();
+                product_columns(tmem + F::kColDv, tmem + F::kColS, s_do + s * F::kTileBytes, idesc_d, i == 0);
+                umma_commit(do_empty + 8 * s);
+                umma_commit(dv_done);
+                if (!(ok = mbar_wait(ds_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull))) break;
+                tc_fence_after();
+                product_columns(tmem + F::kColDk, tmem + F::kColDp, s_q + s * F::kTileBytes, idesc_d, i == 0);
+                umma_commit(q_empty + 8 * s);
+                umma_commit(dk_done);
+                if (i + 1 < items)  // P(i) and dS(i) lie where S(i + 1) and dP(i + 1) go
+                    ok = mbar_wait(dv_done, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && score(i + 1) &&
+                         mbar_wait(dk_done, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && reach(i + 1);
+            }
+            umma_commit(drain);
+            drain_wait(drain, 0, p.status);
+        }
+    } else if (warp < 8) {
+        const int half = warp >> 2;
+        const uint32_t row_base = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+        const int64_t key = k0 + (warp & 3) * 32 + lane;
+        const uint32_t low = warp & 1 ? bits.w[1] : bits.w[0], high = warp & 1 ? bits.w[3] : bits.w[2];
+        const bool on = (warp & 2 ? high : low) >> lane & 1u;
+        const float c = a.scale * kLog2e;
+        const float e2 = grad_exponent<kBf16>(p);
+        constexpr float kP = kBf16 ? 0.0f : 15.0f;  // P is held times 2^kP
+        const float to_ds = kBf16 ? 1.0f : exp2f(e2 - kP);
+        bool ok = true;
+        for (int i = 0; i < items; ++i) {
+            const uint32_t stat = s_stat + (i % F::kStages) * 1024 + half * 256;
+            if (!(ok = mbar_wait_warp(s_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
+            // the copy of -lse completed with the tile that S(i) was made of; this orders it for this thread
+            if (!(ok = mbar_wait_warp(q_full + 8 * (i % F::kStages), (i / F::kStages) & 1, abort_flag, p.status,
+                                      kStatusTimeoutXFull)))
+                break;
+            tc_fence_after();
+            uint32_t r[2][32];
+            tmem_ld32(row_base + F::kColS + half * 64, r[0]);
+            tmem_ld32(row_base + F::kColS + half * 64 + 32, r[1]);
+            tmem_wait_ld32(r[0]);
+            reg_barrier32(r[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    float4 l = ld_shared_f4(stat + (32 * j + e) * 4);
+                    if (!kBf16) l.x += kP, l.y += kP, l.z += kP, l.w += kP;
+                    float x[4] = {__uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]), __uint_as_float(r[j][e + 2]),
+                                  __uint_as_float(r[j][e + 3])};
+                    fma_f32x2(x[0], x[1], c, l.x, l.y);
+                    fma_f32x2(x[2], x[3], c, l.z, l.w);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = exp2_approx(x[k]);
+                    packed[e / 2] = kBf16 ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]);
+                    packed[e / 2 + 1] = kBf16 ? pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]);
+                    if (!kBf16) {
+                        mul_f32x2(x[0], x[1], to_ds, to_ds);
+                        mul_f32x2(x[2], x[3], to_ds, to_ds);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) r[j][e + k] = __float_as_uint(x[k]);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) packed[e] = on ? packed[e] : 0u;
+                tmem_st16(row_base + F::kColS + half * 64 + 16 * j, packed);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full);
+            if (!(ok = mbar_wait_warp(dp_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
+            if (!(ok = mbar_wait_warp(do_full + 8 * (i % F::kStages), (i / F::kStages) & 1, abort_flag, p.status,
+                                      kStatusTimeoutXFull)))
+                break;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t d[32], packed[16];
+                tmem_ld32(row_base + F::kColDp + half * 64 + 32 * j, d);
+                tmem_wait_ld32(d);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 n = ld_shared_f4(stat + 512 + (32 * j + e) * 4);
+                    float x[4] = {__uint_as_float(d[e]), __uint_as_float(d[e + 1]), __uint_as_float(d[e + 2]),
+                                  __uint_as_float(d[e + 3])};
+                    add_f32x2(x[0], x[1], n.x, n.y);
+                    add_f32x2(x[2], x[3], n.z, n.w);
+                    mul_f32x2(x[0], x[1], __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
+                    mul_f32x2(x[2], x[3], __uint_as_float(r[j][e + 2]), __uint_as_float(r[j][e + 3]));
+                    packed[e / 2] = kBf16 ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]);
+                    packed[e / 2 + 1] = kBf16 ? pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) packed[e] = on ? packed[e] : 0u;
+                tmem_st16(row_base + F::kColDp + half * 64 + 16 * j, packed);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_full);
+        }
+        if (items > 0 && ok) ok = mbar_wait_warp(drain, 0, abort_flag, p.status, kStatusTimeoutAccFull);
+        tc_fence_after();
+        // WG 0 writes dV, WG 1 dK
+        const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_len * a.kv_heads;
+        const int64_t row = (b * a.kv_len + key) * a.kv_heads + hk;
+        float* part = a.splits > 1 ? a.part + (2 * split + (half ? 0 : 1)) * rows * a.dim : nullptr;
+        const float f = half ? a.scale * exp2f(-e2) : exp2f(-kP);
+#pragma unroll 1
+        for (int d = 0; d < DP; d += 16) {
+            if (d >= a.dim) break;
+            uint32_t r[16] = {};
+            if (items > 0) {
+                tmem_ld16(row_base + (half ? F::kColDk : F::kColDv) + d, r);
+                tmem_wait_ld(r);
+            }
+            if (ok && key < a.kv_len)
+                store_columns<kBf16>(a, half ? a.dk : a.dv, part, row * a.dim, d, r, f, on && items > 0);
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (warp == 9) {
+        tmem_relinquish();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace attn
+}  // namespace rdvb

@@ -26,7 +26,8 @@ SOURCES = {
                 "exchange.cuh"],
     "norm.cu": ["host.h", "types.cuh", "norm.cuh"],
     "dropout.cu": ["host.h", "types.cuh", "dropout.cuh"],
-    "attention.cu": ["host.h", "types.cuh", "ptx.cuh", "attention.cuh", "attention_tc.cuh"],
+    "attention.cu": ["host.h", "types.cuh", "ptx.cuh", "attention.cuh", "attention_tc.cuh",
+                     "attention_tc_grad.cuh"],
 }
 
 
