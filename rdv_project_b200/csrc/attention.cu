@@ -85,12 +85,24 @@ int encode(TcMap* out, const rdvb_attention* a, const void* base, const int64_t*
 
 int tile_of(const rdvb_attention* a, bool tc) { return tc ? kTcTile : a->dim > 128 ? 32 : 64; }
 
-// Parts into which a launch of `tiles` blocks with `items` loop steps each is
-// split: as many as fill the processors about twice, none of fewer than four
-// steps, at most 32 (their join reads every part).
-int splits_for(int64_t tiles, int64_t items) {
-    const int64_t want = 2 * 148 / std::max<int64_t>(tiles, 1);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, items / 4, 32})));
+// Parts that the long axis is split into: those that make the launch
+// shortest. `blocks` blocks of `steps` loop steps run `slots` at a time, a
+// step takes step_us; parts are written and read once more by a join
+// (part_bytes each, at 6.5 TB/s, and 4 us of launch). At least two steps a
+// part, at most 32 parts.
+int splits_for(int64_t blocks, int64_t steps, int64_t slots, double step_us, double part_bytes) {
+    int best = 1;
+    double least = 0.0;
+    for (int s = 1; s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
+        const double rounds = static_cast<double>(ceil_div(blocks * s, slots));
+        const double us = rounds * static_cast<double>(ceil_div(steps, s)) * step_us +
+                          (s > 1 ? 4.0 + 2.0 * s * part_bytes / 6.5e6 : 0.0);
+        if (s == 1 || us < 0.97 * least) {
+            best = s;
+            least = us;
+        }
+    }
+    return best;
 }
 
 struct Plan {
@@ -107,17 +119,22 @@ Plan plan(const rdvb_attention* a) {
     const int64_t q_tiles = ceil_div(a->q_len, tile), k_tiles = ceil_div(a->kv_len, tile);
     const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
     const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
-    p.forward = splits_for(q_tiles * a->heads * a->batch, k_tiles);
+    // The tensor-core kernels hold one block a processor (the forward one takes two query tiles), the CUDA-core ones
+    // two; a step is a pair of 128 x 128 tiles (measured at about 0.8 and 1.2 us) or of 64 x 64 (about 8 us).
+    const int64_t slots = p.tc ? 148 : 296;
+    const double row_bytes = static_cast<double>(a->dim) * 4;
+    p.forward = splits_for((p.tc ? ceil_div(q_tiles, 2) : q_tiles) * a->heads * a->batch, k_tiles, slots,
+                           p.tc ? 1.2 : 8.0, rows * row_bytes);
     p.forward_len = ceil_div(k_tiles, p.forward) * tile;
     p.forward = static_cast<int>(std::max<int64_t>(1, ceil_div(a->kv_len, std::max<int64_t>(p.forward_len, 1))));
     p.forward_bytes = p.forward > 1 ? round16(p.forward * rows * 8) + p.forward * rows * a->dim * 4 : 0;
     // gradients
     const int64_t bq_tiles = ceil_div(a->q_len, back), bk_tiles = ceil_div(a->kv_len, back);
-    p.dq = splits_for(bq_tiles * a->heads * a->batch, bk_tiles);
+    p.dq = splits_for(bq_tiles * a->heads * a->batch, bk_tiles, slots, p.tc ? 0.8 : 12.0, rows * row_bytes);
     p.dq_len = ceil_div(bk_tiles, p.dq) * back;
     p.dq = static_cast<int>(std::max<int64_t>(1, ceil_div(a->kv_len, std::max<int64_t>(p.dq_len, 1))));
     const int64_t items = bq_tiles * (a->heads / a->kv_heads);
-    p.dkv = splits_for(bk_tiles * a->kv_heads * a->batch, items);
+    p.dkv = splits_for(bk_tiles * a->kv_heads * a->batch, items, slots, p.tc ? 1.2 : 16.0, 2 * kv_rows * row_bytes);
     p.dkv_len = ceil_div(items, p.dkv);
     p.dkv = static_cast<int>(std::max<int64_t>(1, ceil_div(items, std::max<int64_t>(p.dkv_len, 1))));
     p.q_pad = bq_tiles * back;
@@ -172,8 +189,9 @@ int launch(K kernel, int64_t blocks, int smem, const Params& p, cudaStream_t st,
      : a->dim <= 128 ? launch(kernel<128>, __VA_ARGS__ Shape<128>::bytes, p, st, #kernel)                   \
                      : launch(kernel<256>, __VA_ARGS__ Shape<256>::bytes, p, st, #kernel))
 
-int launch_tc_forward(const rdvb_attention* a, const Params& p, int64_t blocks, cudaStream_t st) {
-    if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "tc_forward_kernel: too many blocks");
+int launch_tc_forward(const rdvb_attention* a, const Params& p, const rdvb_host::Device& dev, cudaStream_t st) {
+    const int64_t items = ceil_div(a->q_len, 2 * kTcTile) * a->heads * a->batch * p.splits;
+    if (items > 0x3fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "tc_forward_kernel: too many query tiles");
     TcParams t;
     t.a = p;
     if (int rc = rdvb_host::status_word(&t.status)) return rc;
@@ -188,7 +206,8 @@ int launch_tc_forward(const rdvb_attention* a, const Params& p, int64_t blocks, 
         cudaError_t e =
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-        kernel<<<static_cast<unsigned>(blocks), kTcThreads, smem, st>>>(t, q, k, v);
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, dev.sm_count));
+        kernel<<<grid, kTcThreads, smem, st>>>(t, static_cast<uint32_t>(items), q, k, v);
         return rdvb_host::launched("tc_forward_kernel");
     };
     const bool bf16 = a->dtype == RDVB_BF16;
@@ -303,7 +322,7 @@ int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void*
     p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + round16(p.splits * rows * 8));
     const int64_t blocks = ceil_div(a->q_len, tile_of(a, l.tc)) * a->heads * a->batch * p.splits;
     if (l.tc) {
-        if (int rc = launch_tc_forward(a, p, blocks, st)) return rc;
+        if (int rc = launch_tc_forward(a, p, dev, st)) return rc;
     } else if (int rc = RDVB_BY_DIM(forward_kernel, kForwardBytes, blocks, )) {
         return rc;
     }

@@ -1,15 +1,19 @@
 // Attention (attention.cuh has the mathematics) on the tensor cores, for
 // float16 and bfloat16 with head dimensions up to 128, multiples of 8.
 //
-// A block owns 128 query rows of one head and walks over the keys 128 at a
-// time: S = Q K^T into TMEM (one row a lane), a thread a row takes the
-// running maximum and the exponentials and leaves P, 16 bits an element, in
-// TMEM, and O += P V takes it from there. Q, K and V come by TMA into
-// 128-byte-swizzled tiles; V is the MN-major operand of the second product,
-// so nothing is transposed. Two blocks a processor: while one's warps are in
-// the exponentials the other's products run. Warps 0-3: softmax. Warp 4:
-// loads. Warp 5: products. Warp 6: zeroes the rows of V whose keys are not
-// allowed (their P is 0, but 0 times NaN is not).
+// A block owns two tiles of 128 query rows of one head and walks over the
+// keys 128 at a time: S = Q K^T into TMEM (one row a lane), a thread a row
+// takes the running maximum and the exponentials and leaves P, 16 bits an
+// element, in TMEM, and O += P V takes it from there. Q, K and V come by TMA
+// into 128-byte-swizzled tiles; V is the MN-major operand of the second
+// product, so nothing is transposed. The two tiles take turns: while one's
+// warps are in the exponentials the other's products run, and both read the
+// same K and V. The hardware keeps one block with TMEM on a processor, so a
+// block stays and takes one (head, query tiles) item after another: the next
+// item's first products and loads run beside this one's last rows. Warps 0-3
+// and 4-7: softmax of a tile each. Warp 8: loads. Warp 9: products. Warp 10:
+// zeroes the rows of V whose keys are not allowed (their P is 0, but 0 times
+// NaN is not).
 //
 // S, the row sums and O are float32; P is rounded to the inputs' type, as the
 // tensor cores take it. O is rescaled only when a row's maximum has grown by
@@ -28,10 +32,10 @@ namespace rdvb {
 namespace attn {
 
 constexpr int kTcTile = 128;       // query rows and keys of a tile
-constexpr int kTcThreads = 8 * 32;  // one warp is idle: registers are shared out by groups of four
-// Registers of a thread at launch (two blocks fill a processor's 65,536), and
-// after the softmax warps have taken some of the others' (208 + 48 = 2 x 128).
-constexpr int kTcRegisters = 128, kSoftmaxRegisters = 208, kOtherRegisters = 48;
+constexpr int kTcThreads = 12 * 32;  // one warp is idle: registers are shared out by groups of four
+// Registers of a thread at launch, and after the softmax warps have taken
+// some of the others' (2 x 208 + 88 = 3 x 168).
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 constexpr float kGrowth = 8.0f;    // log2 of the growth of a row's maximum that O is rescaled at
 
 struct TcParams {
@@ -131,6 +135,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// (a0, a1) * (b0, b1) in one packed instruction.
+__device__ __forceinline__ void mul_f32x2(float& a0, float& a1, float b0, float b1) {
+    uint64_t pa, pb, pd;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b0), "f"(b1));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(pd) : "l"(pa), "l"(pb));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
+}
+// (a0 b0 + c0, a1 b1 + c1) in one packed instruction.
+__device__ __forceinline__ void fma_f32x2(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+    uint64_t pa, pb, pc, pd;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b0), "f"(b1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(pc) : "f"(c0), "f"(c1));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(pd) : "l"(pa), "l"(pb), "l"(pc));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
+}
 // (a0 b + c, a1 b + c) in one packed instruction.
 __device__ __forceinline__ void fma_f32x2(float& a0, float& a1, float b, float c) {
     uint64_t pa, pb, pc, pd;
@@ -203,46 +224,110 @@ __device__ __forceinline__ TcPlace tc_place(const Params& p) {
     return t;
 }
 
+// 2^x for x <= 128: x = n + f, |f| <= 1/2, times a polynomial of degree 4 in
+// f with the least largest relative error (2.6e-6, a hundredth of what P is
+// rounded by). Below 2^-126 it is 0, a NaN stays one. It runs on the FMA
+// pipe, beside the exponential unit that ex2 takes.
+__device__ __forceinline__ void exp2_poly2(float& x, float& y) {
+    constexpr float kRound = 12582912.0f + 127.0f;  // adding it leaves n + 127 in the low bits
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x));  // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y));
+    float n0 = x, n1 = y;
+    add_f32x2(n0, n1, kRound, kRound);
+    const float s0 = __uint_as_float(__float_as_uint(n0) << 23), s1 = __uint_as_float(__float_as_uint(n1) << 23);
+    add_f32x2(n0, n1, -kRound, -kRound);
+    float f0 = n0, f1 = n1;
+    fma_f32x2(f0, f1, -1.0f, -1.0f, x, y);
+    float p0 = f0, p1 = f1;
+    fma_f32x2(p0, p1, 0.009570101908f, 0.05591786032f);
+    fma_f32x2(p0, p1, f0, f1, 0.2402474483f, 0.2402474483f);
+    fma_f32x2(p0, p1, f0, f1, 0.6931218147f, 0.6931218147f);
+    fma_f32x2(p0, p1, f0, f1, 0.9999992614f, 0.9999992614f);
+    mul_f32x2(p0, p1, s0, s1);
+    x = p0;
+    y = p1;
+}
+
 template <int DP>
 struct TcForward {
     static constexpr int kAtoms = DP / 64;
     static constexpr uint32_t kTileBytes = kTcTile * DP * 2;
-    static constexpr int kStages = DP == 64 ? 2 : 1;  // K and V tiles in flight; 96 KB either way
-    // TMEM columns: S, O and, where there is room, P beside S instead of over it
+    static constexpr int kStages = DP == 64 ? 3 : 2;  // K and V tiles in flight
+    // TMEM columns: S and O of the two tiles and, where there is room, P beside S instead of over it
     static constexpr bool kOwnP = DP == 64;
-    static constexpr uint32_t kColS = 0, kColO = 128, kColP = kOwnP ? 192 : 0, kCols = 256;
-    static constexpr uint32_t kOffK = kTileBytes, kOffV = kOffK + kStages * kTileBytes,
+    static constexpr uint32_t kColS = 0, kColO = 256, kColP = kOwnP ? 384 : 0, kStepP = kOwnP ? 64 : 128;
+    static constexpr uint32_t kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes,
                               kOffBar = kOffV + kStages * kTileBytes;
     static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // barriers; slack for the 1024-byte alignment
+    // Of eight pairs of exponentials, those taken by the polynomial: at 64
+    // dimensions the exponential unit is what the products wait for.
+    static constexpr int kPolyPairs = DP == 64 ? 2 : 0;
 };
 
+// An item of the forward pass: 256 query rows of one head over the keys of
+// one split.
+struct TcItem {
+    int64_t q0, begin, end;
+    int h, hk, b, split, tiles;
+    bool both;  // the second tile has rows
+};
+__device__ __forceinline__ TcItem tc_item(const Params& p, uint32_t id) {
+    TcItem t;
+    const uint32_t q_items = static_cast<uint32_t>((p.q_len + 2 * kTcTile - 1) / (2 * kTcTile));
+    t.q0 = static_cast<int64_t>(id % q_items) * (2 * kTcTile);
+    id /= q_items;
+    t.h = id % p.heads;
+    id /= p.heads;
+    t.b = id % p.batch;
+    t.split = id / p.batch;
+    t.hk = t.h / p.group;
+    t.both = t.q0 + kTcTile < p.q_len;
+    const int64_t len = length_of(p, t.b);
+    t.begin = t.split * p.split_len;
+    t.end = min(len, t.begin + p.split_len);
+    t.tiles = t.end > t.begin ? static_cast<int>((t.end - t.begin + kTcTile - 1) / kTcTile) : 0;
+    return t;
+}
+
+// The next item of this block with keys, from `id` on; false past the last.
+__device__ __forceinline__ bool next_item(const Params& p, uint32_t items, uint32_t& id, TcItem& t) {
+    for (; id < items; id += gridDim.x) {
+        t = tc_item(p, id);
+        if (t.tiles > 0) return true;
+    }
+    return false;
+}
+
 template <int DP, bool kBf16>
-__global__ void __launch_bounds__(kTcThreads, 2)
-    tc_forward_kernel(const TcParams p, const __grid_constant__ TcMap map_q,
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tc_forward_kernel(const TcParams p, const uint32_t items, const __grid_constant__ TcMap map_q,
                       const __grid_constant__ TcMap map_k, const __grid_constant__ TcMap map_v) {
     using F = TcForward<DP>;
     constexpr int kStages = F::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t s_q = base, s_k = base + F::kOffK, s_v = base + F::kOffV, bars = base + F::kOffBar;
-    const uint32_t q_full = bars, s_full = bars + 8, s_read = bars + 16, p_full = bars + 24, o_full = bars + 32,
-                   drain = bars + 40, k_full = bars + 48, k_empty = bars + 64, v_tma = bars + 80, v_full = bars + 96,
-                   v_empty = bars + 112;
-    const uint32_t tmem_slot = bars + 128;
+    const uint32_t q_full = bars, q_empty = bars + 8, drain = bars + 16, s_full = bars + 24, s_read = bars + 40,
+                   p_full = bars + 56, o_full = bars + 72, o_read = bars + 88, k_full = bars + 104,
+                   k_empty = bars + 128, v_tma = bars + 152, v_full = bars + 176, v_empty = bars + 200;
+    const uint32_t tmem_slot = bars + 224;
     volatile uint32_t* abort_flag =
-        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 132);
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 228);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Params& a = p.a;
-    const TcPlace t = tc_place(a);
 
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
-        mbar_init(q_full, 1);
-        mbar_init(s_full, 1);
-        mbar_init(s_read, 4);
-        mbar_init(p_full, 4);
-        mbar_init(o_full, 1);
+        mbar_init(q_full, 2);  // an arrival a tile
+        mbar_init(q_empty, 1);
         mbar_init(drain, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(s_read + 8 * i, 4);
+            mbar_init(p_full + 8 * i, 4);
+            mbar_init(o_full + 8 * i, 1);
+            mbar_init(o_read + 8 * i, 4);
+        }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(k_full + 8 * i, 1);
             mbar_init(k_empty + 8 * i, 1);
@@ -252,240 +337,307 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         }
         fence_mbarrier_init();
     }
-    if (warp == 5) tmem_alloc(tmem_slot, F::kCols);
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
 
-    if (warp >= 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-    if (warp == 4) {
-        if (lane == 0 && t.tiles > 0) {
-            int k_sent = 0, v_sent = 0;
-            tc_load<F::kAtoms>(s_q, map_q, t.h, t.q0, t.b, q_full);
-            for (int i = 0; i < t.tiles; ++i) {
-                const int s = i % kStages;
-                const uint32_t parity = ((i / kStages) & 1) ^ 1;
-                const int64_t k0 = t.begin + static_cast<int64_t>(i) * kTcTile;
-                if (!mbar_wait(k_empty + 8 * s, parity, abort_flag, p.status, kStatusTimeoutXEmpty)) break;
-                tc_load<F::kAtoms>(s_k + s * F::kTileBytes, map_k, t.hk, k0, t.b, k_full + 8 * s);
-                ++k_sent;
-                if (!mbar_wait(v_empty + 8 * s, parity, abort_flag, p.status, kStatusTimeoutXEmpty)) break;
-                tc_load<F::kAtoms>(s_v + s * F::kTileBytes, map_v, t.hk, k0, t.b, v_tma + 8 * s);
-                ++v_sent;
-            }
-            // no copy may be in flight when the block ends
-            drain_wait(q_full, 0, p.status);
-            for (int s = 0; s < kStages; ++s) {
-                if (k_sent > s) drain_wait(k_full + 8 * s, ((k_sent - 1 - s) / kStages) & 1, p.status);
-                if (v_sent > s) drain_wait(v_tma + 8 * s, ((v_sent - 1 - s) / kStages) & 1, p.status);
-            }
-        }
-    } else if (warp == 5) {
-        if (lane == 0 && t.tiles > 0) {
-            const uint32_t idesc_s = umma_idesc_f16(kTcTile, kBf16);
-            const uint32_t idesc_o = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
-            const uint32_t v_ready = p.guarded ? v_full : v_tma;
-            auto score = [&](int i) {  // S(i) = Q K(i)^T
-                const int s = i % kStages;
-                if (!mbar_wait(k_full + 8 * s, (i / kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull)) return false;
-                tc_fence_after();
-                for (uint32_t j = 0; j < p.k_steps; ++j) {
-                    const uint32_t at = (j >> 2) * (kTcTile * 128) + (j & 3) * 32;
-                    umma_f16(tmem + F::kColS, umma_desc_sw128(s_q + at),
-                             umma_desc_sw128(s_k + s * F::kTileBytes + at), idesc_s, j > 0);
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+        if (warp == 8) {
+            if (lane == 0) {
+                uint32_t n = 0, k_sent = 0, v_sent = 0, q_sent = 0, id = blockIdx.x;  // n: key tiles so far
+                TcItem t;
+                bool ok = true;
+                for (; ok && next_item(a, items, id, t); id += gridDim.x) {
+                    if (!mbar_wait(q_empty, (q_sent & 1) ^ 1, abort_flag, p.status, kStatusTimeoutWEmpty)) break;
+                    ++q_sent;
+                    tc_load<F::kAtoms>(s_q, map_q, t.h, t.q0, t.b, q_full);
+                    if (t.both)
+                        tc_load<F::kAtoms>(s_q + F::kTileBytes, map_q, t.h, t.q0 + kTcTile, t.b, q_full);
+                    else
+                        mbar_arrive(q_full);
+                    for (int i = 0; i < t.tiles; ++i, ++n) {
+                        const uint32_t s = n % kStages, parity = ((n / kStages) & 1) ^ 1;
+                        const int64_t k0 = t.begin + static_cast<int64_t>(i) * kTcTile;
+                        ok = mbar_wait(k_empty + 8 * s, parity, abort_flag, p.status, kStatusTimeoutXEmpty);
+                        if (!ok) break;
+                        tc_load<F::kAtoms>(s_k + s * F::kTileBytes, map_k, t.hk, k0, t.b, k_full + 8 * s);
+                        ++k_sent;
+                        ok = mbar_wait(v_empty + 8 * s, parity, abort_flag, p.status, kStatusTimeoutXEmpty);
+                        if (!ok) break;
+                        tc_load<F::kAtoms>(s_v + s * F::kTileBytes, map_v, t.hk, k0, t.b, v_tma + 8 * s);
+                        ++v_sent;
+                    }
                 }
-                umma_commit(k_empty + 8 * s);
-                umma_commit(s_full);
-                return true;
-            };
-            auto mix = [&](int i) {  // O += P(i) V(i)
-                const int s = i % kStages;
-                if (!mbar_wait(v_ready + 8 * s, (i / kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull)) return false;
-                if (!mbar_wait(p_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull)) return false;
-                tc_fence_after();
+                // no copy may be in flight when the block ends
+                if (q_sent > 0) drain_wait(q_full, (q_sent - 1) & 1, p.status);
+                for (uint32_t s = 0; s < kStages; ++s) {
+                    if (k_sent > s) drain_wait(k_full + 8 * s, ((k_sent - 1 - s) / kStages) & 1, p.status);
+                    if (v_sent > s) drain_wait(v_tma + 8 * s, ((v_sent - 1 - s) / kStages) & 1, p.status);
+                }
+            }
+        } else if (warp == 9) {
+            if (lane == 0) {
+                const uint32_t idesc_s = umma_idesc_f16(kTcTile, kBf16);
+                const uint32_t idesc_o = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
+                const uint32_t v_ready = p.guarded ? v_full : v_tma;
+                // Per query tile: scores and mixes issued, and items whose O was begun.
+                uint32_t scores[2] = {}, mixes[2] = {}, begun[2] = {}, q_items = 0;
+                auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
+                    return mbar_wait(bar, parity & 1, abort_flag, p.status, code);
+                };
+                // S of query tile w with key tile n
+                auto score = [&](int w, uint32_t n) {
+                    const uint32_t s = n % kStages;
+                    if (!wait(k_full + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
+                    if (scores[w] > 0 &&
+                        !wait((F::kOwnP ? s_read : o_full) + 8 * w, scores[w] - 1, kStatusTimeoutAccFull))
+                        return false;  // the softmax has read the last scores; P is not over them or was taken
+                    tc_fence_after();
+                    for (uint32_t j = 0; j < p.k_steps; ++j) {
+                        const uint32_t at = (j >> 2) * (kTcTile * 128) + (j & 3) * 32;
+                        umma_f16(tmem + F::kColS + 128 * w, umma_desc_sw128(s_q + w * F::kTileBytes + at),
+                                 umma_desc_sw128(s_k + s * F::kTileBytes + at), idesc_s, j > 0);
+                    }
+                    umma_commit(s_full + 8 * w);
+                    ++scores[w];
+                    return true;
+                };
+                // O of query tile w += P V with key tile n
+                auto mix = [&](int w, uint32_t n, bool first) {
+                    const uint32_t s = n % kStages;
+                    if (!wait(v_ready + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
+                    if (first && begun[w]++ > 0 && !wait(o_read + 8 * w, begun[w] - 2, kStatusTimeoutDrain))
+                        return false;
+                    if (!wait(p_full + 8 * w, mixes[w], kStatusTimeoutAFull)) return false;
+                    tc_fence_after();
 #pragma unroll
-                for (uint32_t j = 0; j < kTcTile / 16; ++j)
-                    umma_f16_ts(tmem + F::kColO, tmem + F::kColP + 8 * j,
-                                umma_desc_mn_sw128(s_v + s * F::kTileBytes + j * 2048, kTcTile * 128), idesc_o,
-                                i > 0 || j > 0);
-                umma_commit(v_empty + 8 * s);
-                umma_commit(o_full);
-                return true;
-            };
-            bool ok = mbar_wait(q_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0);
-            for (int i = 0; ok && i < t.tiles; ++i) {
-                if (F::kOwnP) {
-                    // the next scores may start when the softmax has read these
-                    if (i + 1 < t.tiles)
-                        ok = mbar_wait(s_read, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && score(i + 1);
-                    ok = ok && mix(i);
-                } else {
-                    ok = mix(i);
-                    // P(i) lies where S(i + 1) goes
-                    if (ok && i + 1 < t.tiles)
-                        ok = mbar_wait(o_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && score(i + 1);
+                    for (uint32_t j = 0; j < kTcTile / 16; ++j)
+                        umma_f16_ts(tmem + F::kColO + DP * w, tmem + F::kColP + F::kStepP * w + 8 * j,
+                                    umma_desc_mn_sw128(s_v + s * F::kTileBytes + j * 2048, kTcTile * 128), idesc_o,
+                                    !first || j > 0);
+                    umma_commit(o_full + 8 * w);
+                    ++mixes[w];
+                    return true;
+                };
+                uint32_t id = blockIdx.x, n = 0;
+                TcItem t, u;
+                bool ok = true, have = next_item(a, items, id, t);
+                // scores of the step (item v, its key tile i, key tile n of the block), query tile w
+                auto ahead = [&](const TcItem& v, int i, uint32_t n, int w) {
+                    if (w && !v.both) return true;
+                    if (w == 0 && i == 0 && !wait(q_full, q_items++, kStatusTimeoutWFull)) return false;
+                    if (!score(w, n)) return false;
+                    if (w == (v.both ? 1 : 0)) {
+                        umma_commit(k_empty + 8 * (n % kStages));
+                        if (i == v.tiles - 1) umma_commit(q_empty);
+                    }
+                    return true;
+                };
+                if (have) ok = ahead(t, 0, 0, 0) && ahead(t, 0, 0, 1);
+                while (ok && have) {
+                    // u: the item after t
+                    uint32_t next = id + gridDim.x;
+                    const bool more = next_item(a, items, next, u);
+                    for (int i = 0; ok && i < t.tiles; ++i, ++n) {
+                        const bool within = i + 1 < t.tiles;
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            if (F::kOwnP && ok && (within || more)) ok = ahead(within ? t : u, within ? i + 1 : 0, n + 1, w);
+                            if (ok && (w == 0 || t.both)) {
+                                ok = mix(w, n, i == 0);
+                                if (w == (t.both ? 1 : 0)) umma_commit(v_empty + 8 * (n % kStages));
+                            }
+                            if (!F::kOwnP && ok && (within || more)) ok = ahead(within ? t : u, within ? i + 1 : 0, n + 1, w);
+                        }
+                    }
+                    have = more;
+                    t = u;
+                    id = next;
                 }
+                umma_commit(drain);
+                drain_wait(drain, 0, p.status);
             }
-            umma_commit(drain);
-            drain_wait(drain, 0, p.status);
-        }
-    } else if (warp == 6) {
-        if (p.guarded) {
-            for (int i = 0; i < t.tiles; ++i) {
-                const int s = i % kStages;
-                const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
-                if (!mbar_wait_warp(v_tma + 8 * s, (i / kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull)) break;
-                if (!bits.all()) {
-                    zero_rows<F::kAtoms>(s_v + s * F::kTileBytes, bits);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
-                if (lane == 0) mbar_arrive(v_full + 8 * s);
+        } else if (warp == 10) {
+            if (p.guarded) {
+                uint32_t n = 0, id = blockIdx.x;
+                TcItem t;
+                bool ok = true;
+                for (; ok && next_item(a, items, id, t); id += gridDim.x)
+                    for (int i = 0; i < t.tiles; ++i, ++n) {
+                        const uint32_t s = n % kStages;
+                        const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+                        ok = mbar_wait_warp(v_tma + 8 * s, (n / kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull);
+                        if (!ok) break;
+                        if (!bits.all()) {
+                            zero_rows<F::kAtoms>(s_v + s * F::kTileBytes, bits);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                        if (lane == 0) mbar_arrive(v_full + 8 * s);
+                    }
             }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-        const uint32_t row_base = tmem + (static_cast<uint32_t>(warp) << 21);  // lane 32 * warp of TMEM
+        const int w = warp >> 2;
+        const uint32_t row_base = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // lane 32 (warp % 4) of TMEM
+        const uint32_t col_s = row_base + F::kColS + 128 * w, col_o = row_base + F::kColO + DP * w,
+                       col_p = row_base + F::kColP + F::kStepP * w;
         const float c = a.scale * kLog2e;
-        float top = -INFINITY, total = 0.0f;
-        bool any = false, ok = true;
-        for (int i = 0; i < t.tiles; ++i) {
-            const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
-            const bool whole = bits.all();
-            any |= !bits.none();
-            if (!(ok = mbar_wait_warp(s_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
-            tc_fence_after();
-            uint32_t r[8][16];
+        uint32_t n = 0;  // key tiles of this query tile so far
+        bool ok = true;
+        for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+            const TcItem t = tc_item(a, id);
+            if (w && !t.both) continue;
+            float top = -INFINITY, total = 0.0f;
+            bool any = false;
+            for (int i = 0; i < t.tiles; ++i, ++n) {
+                const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+                const bool whole = bits.all();
+                any |= !bits.none();
+                if (!(ok = mbar_wait_warp(s_full + 8 * w, n & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
+                tc_fence_after();
+                uint32_t r[8][16];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) tmem_ld16(row_base + F::kColS + 16 * j, r[j]);
-            tmem_wait_ld(r[0]);
+                for (int j = 0; j < 8; ++j) tmem_ld16(col_s + 16 * j, r[j]);
+                tmem_wait_ld(r[0]);
 #pragma unroll
-            for (int j = 1; j < 8; ++j) reg_barrier(r[j]);
-            if (F::kOwnP) {  // S has been read
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_read);
-            }
-            if (!whole) {
+                for (int j = 1; j < 8; ++j) reg_barrier(r[j]);
+                if (F::kOwnP) {  // S has been read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_read + 8 * w);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            r[j][e] = bits.w[j / 2] >> (j % 2 * 16 + e) & 1u ? r[j][e] : 0xff800000u;
+                }
+                float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        r[j][e] = bits.w[j / 2] >> (j % 2 * 16 + e) & 1u ? r[j][e] : 0xff800000u;
-            }
-            float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2)
-                    high[j & 3] = fmaxf(fmaxf(high[j & 3], __uint_as_float(r[j][e])), __uint_as_float(r[j][e + 1]));
-            const float m = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * c;
-            const bool grows = m > top + kGrowth || (top == -INFINITY && m > -INFINITY);
-            if (i > 0 && !mbar_wait_warp(o_full, (i - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull)) {
-                ok = false;
-                break;
-            }
-            if (__any_sync(0xffffffffu, grows)) {
-                const float fresh = grows ? m : top;
-                const float f = fresh == -INFINITY ? 1.0f : exp2_approx(top - fresh);
-                total *= f;
-                top = fresh;
-                if (i > 0) {
-                    tc_fence_after();
+                    for (int e = 0; e < 16; e += 2)
+                        high[j & 3] = fmaxf(fmaxf(high[j & 3], __uint_as_float(r[j][e])), __uint_as_float(r[j][e + 1]));
+                const float m = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * c;
+                const bool grows = m > top + kGrowth || (top == -INFINITY && m > -INFINITY);
+                // the last product has read P and written O
+                if (i > 0 && !mbar_wait_warp(o_full + 8 * w, (n - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull)) {
+                    ok = false;
+                    break;
+                }
+                if (__any_sync(0xffffffffu, grows)) {
+                    const float fresh = grows ? m : top;
+                    const float f = fresh == -INFINITY ? 1.0f : exp2_approx(top - fresh);
+                    total *= f;
+                    top = fresh;
+                    if (i > 0) {
+                        tc_fence_after();
 #pragma unroll 1
-                    for (uint32_t j = 0; j < p.n_pv; j += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(row_base + F::kColO + j, o);
-                        tmem_wait_ld(o);
+                        for (uint32_t j = 0; j < p.n_pv; j += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(col_o + j, o);
+                            tmem_wait_ld(o);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st16(row_base + F::kColO + j, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st8(col_o + j, *reinterpret_cast<uint32_t(*)[8]>(&o[0]));
+                            tmem_st8(col_o + j + 8, *reinterpret_cast<uint32_t(*)[8]>(&o[8]));
+                        }
+                    }
+                }
+                const float minus = top == -INFINITY ? 0.0f : -top;
+                float sum[4] = {};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t packed[8];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
+                        fma_f32x2(x, y, c, minus);
+                        if (e / 2 % 4 == 3 && F::kPolyPairs > e / 8) {
+                            exp2_poly2(x, y);
+                        } else {
+                            x = exp2_approx(x);
+                            y = exp2_approx(y);
+                        }
+                        add_f32x2(sum[e & 2], sum[(e & 2) + 1], x, y);
+                        packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                    }
+                    tmem_st8(col_p + 8 * j, packed);
+                }
+                total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * w);
+            }
+            if (t.tiles > 0 && ok)
+                ok = mbar_wait_warp(o_full + 8 * w, (n - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t q = t.q0 + threadIdx.x;  // 128 rows a tile: warps 4-7 are its second half
+            const bool mine = q < a.q_len;
+            const int64_t row = (t.b * a.q_len + q) * a.heads + t.h;
+            const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;
+            const float inv = any ? 1.0f / total : 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < a.dim; j += 16) {
+                uint32_t r[16] = {};
+                if (t.tiles > 0) {
+                    tmem_ld16(col_o + j, r);
+                    tmem_wait_ld(r);
+                }
+                if (!mine) continue;
+                if (a.splits > 1) {
+                    float* dst = a.part + (t.split * rows + row) * a.dim + j;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (j + e < a.dim)
+                            *reinterpret_cast<uint4*>(dst + e) =
+                                any ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]) : make_uint4(0, 0, 0, 0);
+                } else {
+                    uint16_t* dst = static_cast<uint16_t*>(a.o) + row * a.dim + j;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float x = __uint_as_float(r[e + 2 * k]) * inv,
+                                        y = __uint_as_float(r[e + 2 * k + 1]) * inv;
+                            v[k] = !any ? 0u : kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                        }
+                        if (j + e < a.dim) *reinterpret_cast<uint4*>(dst + e) = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 }
             }
-            const float minus = top == -INFINITY ? 0.0f : -top;
-            float sum[4] = {};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t packed[8];
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
-                    fma_f32x2(x, y, c, minus);
-                    x = exp2_approx(x);
-                    y = exp2_approx(y);
-                    add_f32x2(sum[e & 2], sum[(e & 2) + 1], x, y);
-                    packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+            if (t.tiles > 0) {  // the next item may begin its O
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_read + 8 * w);
+            }
+            if (mine) {
+                if (a.splits > 1) {
+                    a.part_stat[2 * (t.split * rows + row)] = top;
+                    a.part_stat[2 * (t.split * rows + row) + 1] = any ? total : -1.0f;
+                } else if (a.lse) {
+                    a.lse[(static_cast<int64_t>(t.b) * a.heads + t.h) * a.q_len + q] =
+                        any ? (top + log2f(total)) * kLn2 : -INFINITY;
                 }
-                tmem_st8(row_base + F::kColP + 8 * j, packed);
-            }
-            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
-        }
-        if (t.tiles > 0 && ok)
-            ok = mbar_wait_warp(o_full, (t.tiles - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull);
-        tc_fence_after();
-        const int64_t q = t.q0 + threadIdx.x;
-        const bool mine = q < a.q_len && ok;
-        const int64_t row = (t.b * a.q_len + q) * a.heads + t.h;
-        const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;
-        const float inv = any ? 1.0f / total : 0.0f;
-#pragma unroll 1
-        for (int j = 0; j < DP / 32; ++j) {
-            if (32 * j >= a.dim) break;
-            uint32_t r[32];
-            if (t.tiles > 0) {
-                tmem_ld32(row_base + F::kColO + 32 * j, r);
-                tmem_wait_ld32(r);
-            }
-            if (!any) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) r[e] = 0u;
-            }
-            if (!mine) continue;
-            if (a.splits > 1) {
-                float* dst = a.part + (t.split * rows + row) * a.dim + 32 * j;
-#pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    if (32 * j + e < a.dim)
-                        *reinterpret_cast<uint4*>(dst + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
-            } else {
-                uint16_t* dst = static_cast<uint16_t*>(a.o) + row * a.dim + 32 * j;
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float x = __uint_as_float(r[e + 2 * k]) * inv, y = __uint_as_float(r[e + 2 * k + 1]) * inv;
-                        w[k] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
-                    }
-                    if (32 * j + e < a.dim) *reinterpret_cast<uint4*>(dst + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
-        if (mine) {
-            if (a.splits > 1) {
-                a.part_stat[2 * (t.split * rows + row)] = top;
-                a.part_stat[2 * (t.split * rows + row) + 1] = any ? total : -1.0f;
-            } else if (a.lse) {
-                a.lse[(static_cast<int64_t>(t.b) * a.heads + t.h) * a.q_len + q] =
-                    any ? (top + log2f(total)) * kLn2 : -INFINITY;
             }
         }
     }
     tc_fence_before();
     __syncwarp();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == 9) {
         tmem_relinquish();
-        tmem_dealloc(tmem, F::kCols);
+        tmem_dealloc(tmem, 512);
     }
 }
 

@@ -137,23 +137,6 @@ __device__ __forceinline__ float grad_exponent(const GradParams& p) {
     return fminf(fmaxf(floorf(15.0f - log2f(bound)), -100.0f), 100.0f);
 }
 
-// (a0, a1) * (b0, b1) in one packed instruction.
-__device__ __forceinline__ void mul_f32x2(float& a0, float& a1, float b0, float b1) {
-    uint64_t pa, pb, pd;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b0), "f"(b1));
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(pd) : "l"(pa), "l"(pb));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
-}
-// (a0 b + c0, a1 b + c1) in one packed instruction.
-__device__ __forceinline__ void fma_f32x2(float& a0, float& a1, float b, float c0, float c1) {
-    uint64_t pa, pb, pc, pd;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(pb) : "f"(b));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pc) : "f"(c0), "f"(c1));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(pd) : "l"(pa), "l"(pb), "l"(pc));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
-}
 __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -602,8 +585,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                     if (!kBf16) l.x += kP, l.y += kP, l.z += kP, l.w += kP;
                     float x[4] = {__uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]), __uint_as_float(r[j][e + 2]),
                                   __uint_as_float(r[j][e + 3])};
-                    fma_f32x2(x[0], x[1], c, l.x, l.y);
-                    fma_f32x2(x[2], x[3], c, l.z, l.w);
+                    fma_f32x2(x[0], x[1], c, c, l.x, l.y);
+                    fma_f32x2(x[2], x[3], c, c, l.z, l.w);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) x[k] = exp2_approx(x[k]);
                     packed[e / 2] = kBf16 ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]);
