@@ -11,9 +11,10 @@
 // same K and V. The hardware keeps one block with TMEM on a processor, so a
 // block stays and takes one (head, query tiles) item after another: the next
 // item's first products and loads run beside this one's last rows. Warps 0-3
-// and 4-7: softmax of a tile each. Warp 8: loads. Warp 9: products. Warp 10:
-// zeroes the rows of V whose keys are not allowed (their P is 0, but 0 times
-// NaN is not).
+// and 4-7: softmax of a tile each. Warp 8: loads. Warps 9 and 11: products of
+// a tile each (a single issuing thread was the bound: 24 to 32 products and
+// their waits took it about 4,900 cycles a pair of tiles). Warp 10: zeroes the
+// rows of V whose keys are not allowed (their P is 0, but 0 times NaN is not).
 //
 // S, the row sums and O are float32; P is rounded to the inputs' type, as the
 // tensor cores take it. O is rescaled only when a row's maximum has grown by
@@ -32,7 +33,7 @@ namespace rdvb {
 namespace attn {
 
 constexpr int kTcTile = 128;       // query rows and keys of a tile
-constexpr int kTcThreads = 12 * 32;  // one warp is idle: registers are shared out by groups of four
+constexpr int kTcThreads = 12 * 32;
 // Registers of a thread at launch, and after the softmax warps have taken
 // some of the others' (2 x 208 + 88 = 3 x 168).
 constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
@@ -63,19 +64,50 @@ __device__ __forceinline__ void tc_load(uint32_t dst, const TcMap& m, int head, 
                     sample * m.batch_step, bar);
 }
 
-// The 128-byte-swizzled MN-major operand of 16-bit elements: rows of 64 n
-// elements (128 bytes) per k, 8-k groups 1024 bytes apart, the next 64 n
-// elements `lbo` bytes on. 16 k are 2048 bytes.
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t lbo) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;
-    d |= static_cast<uint64_t>(2u) << 61;
-    return d;
+// Shared-memory operands of a product in two words: the low one holds the
+// address (16-byte units, 14 bits), so that a step along K is an addition.
+// K-major, 128-byte swizzle: rows of 64 elements, 8-row groups 1024 bytes
+// apart; 16 k are 32 bytes. MN-major, 128-byte swizzle: rows of 64 n elements
+// per k, 8-k groups 1024 bytes apart, the next 64 n elements a tile (16 KB)
+// on; 16 k are 2048 bytes.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t saddr) {
+    return (saddr >> 4) | ((kTcTile * 128u >> 4) << 16);
 }
 constexpr uint32_t kIdescBTransposed = 1u << 16;
+
+// D (+)= A B^T with both operands in shared memory, one K step of 16.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 x, {%1, %3};\n\t"
+        "mov.b64 y, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// The same with A in TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 y, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// D = A B^T, both K-major tiles of 128 rows (descriptors of their starts),
+// `steps` of at most kMost steps of 16.
+template <int kMost>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t steps, uint32_t idesc) {
+#pragma unroll
+    for (uint32_t j = 0; j < kMost; ++j) {
+        const uint32_t at = (j >> 2) * (kTcTile * 128 / 16) + (j & 3) * 2;
+        if (j < steps) umma_ss(d, a + at, b + at, idesc, j > 0);
+    }
+}
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -255,6 +287,7 @@ struct TcForward {
     static constexpr int kStages = DP == 64 ? 3 : 2;  // K and V tiles in flight
     // TMEM columns: S and O of the two tiles and, where there is room, P beside S instead of over it
     static constexpr bool kOwnP = DP == 64;
+    static constexpr int kIssuers = DP == 64 ? 2 : 1;
     static constexpr uint32_t kColS = 0, kColO = 256, kColP = kOwnP ? 384 : 0, kStepP = kOwnP ? 64 : 128;
     static constexpr uint32_t kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes,
                               kOffBar = kOffV + kStages * kTileBytes;
@@ -267,14 +300,14 @@ struct TcForward {
 // An item of the forward pass: 256 query rows of one head over the keys of
 // one split.
 struct TcItem {
-    int64_t q0, begin, end;
+    int q0, begin, end;  // positions fit 31 bits
     int h, hk, b, split, tiles;
     bool both;  // the second tile has rows
 };
 __device__ __forceinline__ TcItem tc_item(const Params& p, uint32_t id) {
     TcItem t;
     const uint32_t q_items = static_cast<uint32_t>((p.q_len + 2 * kTcTile - 1) / (2 * kTcTile));
-    t.q0 = static_cast<int64_t>(id % q_items) * (2 * kTcTile);
+    t.q0 = static_cast<int>(id % q_items) * (2 * kTcTile);
     id /= q_items;
     t.h = id % p.heads;
     id /= p.heads;
@@ -282,10 +315,10 @@ __device__ __forceinline__ TcItem tc_item(const Params& p, uint32_t id) {
     t.split = id / p.batch;
     t.hk = t.h / p.group;
     t.both = t.q0 + kTcTile < p.q_len;
-    const int64_t len = length_of(p, t.b);
-    t.begin = t.split * p.split_len;
-    t.end = min(len, t.begin + p.split_len);
-    t.tiles = t.end > t.begin ? static_cast<int>((t.end - t.begin + kTcTile - 1) / kTcTile) : 0;
+    const int64_t len = length_of(p, t.b), begin = t.split * p.split_len, end = min(len, begin + p.split_len);
+    t.begin = static_cast<int>(begin);
+    t.end = static_cast<int>(end);
+    t.tiles = end > begin ? static_cast<int>((end - begin + kTcTile - 1) / kTcTile) : 0;
     return t;
 }
 
@@ -319,8 +352,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
         mbar_init(q_full, 2);  // an arrival a tile
-        mbar_init(q_empty, 1);
-        mbar_init(drain, 1);
+        mbar_init(q_empty, 2);  // the empty barriers: an arrival a query tile
+        mbar_init(drain, F::kIssuers);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
             mbar_init(s_read + 8 * i, 4);
@@ -330,10 +363,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(k_full + 8 * i, 1);
-            mbar_init(k_empty + 8 * i, 1);
+            mbar_init(k_empty + 8 * i, 2);
             mbar_init(v_tma + 8 * i, 1);
             mbar_init(v_full + 8 * i, 1);
-            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(v_empty + 8 * i, 2);
         }
         fence_mbarrier_init();
     }
@@ -379,79 +412,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (v_sent > s) drain_wait(v_tma + 8 * s, ((v_sent - 1 - s) / kStages) & 1, p.status);
                 }
             }
-        } else if (warp == 9) {
+        } else if (warp == 9 || (warp == 11 && F::kIssuers == 2)) {
             if (lane == 0) {
+                // Products of query tile w: of both, or of this warp's own. Where an item has no second tile the
+                // first one's releases count twice.
+                const int w0 = F::kIssuers == 2 && warp == 11 ? 1 : 0;
+                constexpr int kMine = F::kIssuers == 2 ? 1 : 2;
                 const uint32_t idesc_s = umma_idesc_f16(kTcTile, kBf16);
                 const uint32_t idesc_o = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
                 const uint32_t v_ready = p.guarded ? v_full : v_tma;
-                // Per query tile: scores and mixes issued, and items whose O was begun.
-                uint32_t scores[2] = {}, mixes[2] = {}, begun[2] = {}, q_items = 0;
+                const uint32_t q_desc = desc_k_major(s_q), k_desc = desc_k_major(s_k), v_desc = desc_mn_major(s_v);
+                uint32_t scores[kMine] = {}, begun[kMine] = {};  // S issued (P V: one less or as many), O begun
                 auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
                     return mbar_wait(bar, parity & 1, abort_flag, p.status, code);
                 };
-                // S of query tile w with key tile n
-                auto score = [&](int w, uint32_t n) {
-                    const uint32_t s = n % kStages;
-                    if (!wait(k_full + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
-                    if (scores[w] > 0 &&
-                        !wait((F::kOwnP ? s_read : o_full) + 8 * w, scores[w] - 1, kStatusTimeoutAccFull))
-                        return false;  // the softmax has read the last scores; P is not over them or was taken
+                auto release = [&](uint32_t bar, bool both) {
+                    umma_commit(bar);
+                    if (!both) umma_commit(bar);
+                };
+                // S of key tile i (the block's n-th) of item v, its query_item-th
+                auto score = [&](int m, const TcItem& v, int i, uint32_t n, uint32_t query_item) {
+                    const uint32_t s = n % kStages, w = w0 + m;
+                    if (i == 0 && m == 0 && !wait(q_full, query_item, kStatusTimeoutWFull)) return false;
+                    if (m == 0 && !wait(k_full + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
+                    // the softmax has read the last scores, and P does not lie over them or was taken
+                    if (scores[m] > 0 &&
+                        !wait((F::kOwnP ? s_read : o_full) + 8 * w, scores[m] - 1, kStatusTimeoutAccFull))
+                        return false;
                     tc_fence_after();
-                    for (uint32_t j = 0; j < p.k_steps; ++j) {
-                        const uint32_t at = (j >> 2) * (kTcTile * 128) + (j & 3) * 32;
-                        umma_f16(tmem + F::kColS + 128 * w, umma_desc_sw128(s_q + w * F::kTileBytes + at),
-                                 umma_desc_sw128(s_k + s * F::kTileBytes + at), idesc_s, j > 0);
-                    }
+                    product_rows<DP / 16>(tmem + F::kColS + 128 * w, q_desc + w * (F::kTileBytes / 16),
+                                          k_desc + s * (F::kTileBytes / 16), p.k_steps, idesc_s);
                     umma_commit(s_full + 8 * w);
-                    ++scores[w];
+                    ++scores[m];
+                    release(k_empty + 8 * s, v.both);
+                    if (i == v.tiles - 1) release(q_empty, v.both);
                     return true;
                 };
-                // O of query tile w += P V with key tile n
-                auto mix = [&](int w, uint32_t n, bool first) {
-                    const uint32_t s = n % kStages;
-                    if (!wait(v_ready + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
-                    if (first && begun[w]++ > 0 && !wait(o_read + 8 * w, begun[w] - 2, kStatusTimeoutDrain))
+                // O += P V with the block's n-th key tile; `mixes` before it
+                auto mix = [&](int m, const TcItem& v, int i, uint32_t n, uint32_t mixes) {
+                    const uint32_t s = n % kStages, w = w0 + m;
+                    if (m == 0 && !wait(v_ready + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
+                    if (i == 0 && begun[m]++ > 0 && !wait(o_read + 8 * w, begun[m] - 2, kStatusTimeoutDrain))
                         return false;
-                    if (!wait(p_full + 8 * w, mixes[w], kStatusTimeoutAFull)) return false;
+                    if (!wait(p_full + 8 * w, mixes, kStatusTimeoutAFull)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (uint32_t j = 0; j < kTcTile / 16; ++j)
-                        umma_f16_ts(tmem + F::kColO + DP * w, tmem + F::kColP + F::kStepP * w + 8 * j,
-                                    umma_desc_mn_sw128(s_v + s * F::kTileBytes + j * 2048, kTcTile * 128), idesc_o,
-                                    !first || j > 0);
+                        umma_ts(tmem + F::kColO + DP * w, tmem + F::kColP + F::kStepP * w + 8 * j,
+                                v_desc + s * (F::kTileBytes / 16) + 128 * j, idesc_o, i > 0 || j > 0);
                     umma_commit(o_full + 8 * w);
-                    ++mixes[w];
+                    release(v_empty + 8 * s, v.both);
                     return true;
                 };
-                uint32_t id = blockIdx.x, n = 0;
+                uint32_t id = blockIdx.x, n = 0, query_items = 0;
                 TcItem t, u;
                 bool ok = true, have = next_item(a, items, id, t);
-                // scores of the step (item v, its key tile i, key tile n of the block), query tile w
-                auto ahead = [&](const TcItem& v, int i, uint32_t n, int w) {
-                    if (w && !v.both) return true;
-                    if (w == 0 && i == 0 && !wait(q_full, q_items++, kStatusTimeoutWFull)) return false;
-                    if (!score(w, n)) return false;
-                    if (w == (v.both ? 1 : 0)) {
-                        umma_commit(k_empty + 8 * (n % kStages));
-                        if (i == v.tiles - 1) umma_commit(q_empty);
-                    }
-                    return true;
-                };
-                if (have) ok = ahead(t, 0, 0, 0) && ahead(t, 0, 0, 1);
+#pragma unroll
+                for (int m = 0; m < kMine; ++m)
+                    if (ok && have && (w0 + m == 0 || t.both)) ok = score(m, t, 0, 0, 0);
                 while (ok && have) {
-                    // u: the item after t
-                    uint32_t next = id + gridDim.x;
+                    uint32_t next = id + gridDim.x;  // u: the item after t
                     const bool more = next_item(a, items, next, u);
+                    ++query_items;
                     for (int i = 0; ok && i < t.tiles; ++i, ++n) {
                         const bool within = i + 1 < t.tiles;
 #pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            if (F::kOwnP && ok && (within || more)) ok = ahead(within ? t : u, within ? i + 1 : 0, n + 1, w);
-                            if (ok && (w == 0 || t.both)) {
-                                ok = mix(w, n, i == 0);
-                                if (w == (t.both ? 1 : 0)) umma_commit(v_empty + 8 * (n % kStages));
-                            }
-                            if (!F::kOwnP && ok && (within || more)) ok = ahead(within ? t : u, within ? i + 1 : 0, n + 1, w);
+                        for (int m = 0; m < kMine; ++m) {
+                            const bool here = w0 + m == 0 || t.both;
+                            const bool ahead = within ? here : more && (w0 + m == 0 || u.both);
+                            const uint32_t mixes = scores[m] - 1;
+                            if (F::kOwnP && ok && ahead)
+                                ok = within ? score(m, t, i + 1, n + 1, query_items - 1)
+                                            : score(m, u, 0, n + 1, query_items);
+                            if (ok && here) ok = mix(m, t, i, n, mixes);
+                            if (!F::kOwnP && ok && ahead)
+                                ok = within ? score(m, t, i + 1, n + 1, query_items - 1)
+                                            : score(m, u, 0, n + 1, query_items);
                         }
                     }
                     have = more;
@@ -581,7 +617,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = mbar_wait_warp(o_full + 8 * w, (n - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull);
             if (!ok) break;
             tc_fence_after();
-            const int64_t q = t.q0 + threadIdx.x;  // 128 rows a tile: warps 4-7 are its second half
+            const int64_t q = t.q0 + static_cast<int>(threadIdx.x);  // 128 rows a tile: warps 4-7 are its second half
             const bool mine = q < a.q_len;
             const int64_t row = (t.b * a.q_len + q) * a.heads + t.h;
             const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;

@@ -146,20 +146,12 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
     return v;
 }
 
-// D += A B^T with both operands K-major tiles of 128 rows (S, dP), fresh.
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t steps, uint32_t idesc) {
-    for (uint32_t j = 0; j < steps; ++j) {
-        const uint32_t at = (j >> 2) * (kTcTile * 128) + (j & 3) * 32;
-        umma_f16(d, umma_desc_sw128(a + at), umma_desc_sw128(b + at), idesc, j > 0);
-    }
-}
 // D += A B with A in TMEM in two halves 64 columns apart (P, dS), B a tile
 // of 128 rows taken along them.
 __device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool first) {
 #pragma unroll
     for (uint32_t j = 0; j < kTcTile / 16; ++j)
-        umma_f16_ts(d, a + (j >> 2) * 64 + (j & 3) * 8, umma_desc_mn_sw128(b + j * 2048, kTcTile * 128), idesc,
-                    !first || j > 0);
+        umma_ts(d, a + (j >> 2) * 64 + (j & 3) * 8, b + j * 128, idesc, !first || j > 0);
 }
 
 // Stores 16 columns of a gradient row from accumulators: 16-bit, or float32
@@ -279,7 +271,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 if (!mbar_wait(k_ready + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows(tmem + F::kColS + (i & 1) * 128, s_q, s_k + s * F::kTileBytes, p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::kColS + (i & 1) * 128, desc_k_major(s_q),
+                                      desc_k_major(s_k + s * F::kTileBytes), p.k_steps, idesc);
                 umma_commit(s_full + 8 * (i & 1));
                 return true;
             };
@@ -288,7 +281,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 if (!mbar_wait(v_full + 8 * s, (i / F::kVStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows(tmem + F::kColDp, s_do, s_v + s * F::kTileBytes, p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::kColDp, desc_k_major(s_do), desc_k_major(s_v + s * F::kTileBytes),
+                                      p.k_steps, idesc);
                 umma_commit(v_empty + 8 * s);
                 umma_commit(dp_full);
                 return true;
@@ -300,8 +294,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 ok = mbar_wait(ds_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull);
                 if (!ok) break;
                 tc_fence_after();
-                product_columns(tmem + F::kColDq, tmem + F::kColS + (i & 1) * 128, s_k + s * F::kTileBytes, idesc_q,
-                                i == 0);
+                product_columns(tmem + F::kColDq, tmem + F::kColS + (i & 1) * 128,
+                                desc_mn_major(s_k + s * F::kTileBytes), idesc_q, i == 0);
                 umma_commit(k_empty + 8 * s);
                 umma_commit(dq_done);
                 if (i + 1 < t.tiles) ok = reach(i + 1);  // dP(i) was read before ds_full
@@ -519,7 +513,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 if (!mbar_wait(q_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows(tmem + F::kColS, s_k, s_q + s * F::kTileBytes, p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::kColS, desc_k_major(s_k), desc_k_major(s_q + s * F::kTileBytes),
+                                      p.k_steps, idesc);
                 umma_commit(s_full);
                 return true;
             };
@@ -528,7 +523,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 if (!mbar_wait(do_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows(tmem + F::kColDp, s_v, s_do + s * F::kTileBytes, p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::kColDp, desc_k_major(s_v), desc_k_major(s_do + s * F::kTileBytes),
+                                      p.k_steps, idesc);
                 umma_commit(dp_full);
                 return true;
             };
@@ -537,12 +533,14 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 const int s = i % F::kStages;
                 if (!(ok = mbar_wait(p_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull))) break;
                 tc_fence_after();
-                product_columns(tmem + F::kColDv, tmem + F::kColS, s_do + s * F::kTileBytes, idesc_d, i == 0);
+                product_columns(tmem + F::kColDv, tmem + F::kColS, desc_mn_major(s_do + s * F::kTileBytes), idesc_d,
+                                i == 0);
                 umma_commit(do_empty + 8 * s);
                 umma_commit(dv_done);
                 if (!(ok = mbar_wait(ds_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull))) break;
                 tc_fence_after();
-                product_columns(tmem + F::kColDk, tmem + F::kColDp, s_q + s * F::kTileBytes, idesc_d, i == 0);
+                product_columns(tmem + F::kColDk, tmem + F::kColDp, desc_mn_major(s_q + s * F::kTileBytes), idesc_d,
+                                i == 0);
                 umma_commit(q_empty + 8 * s);
                 umma_commit(dk_done);
                 if (i + 1 < items)  // P(i) and dS(i) lie where S(i + 1) and dP(i + 1) go
