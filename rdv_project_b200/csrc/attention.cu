@@ -7,6 +7,7 @@
 #include "attention.cuh"
 #include "attention_tc.cuh"
 #include "attention_tc_grad.cuh"
+#include "attention_few.cuh"
 #include "host.h"
 
 using rdvb_host::aligned;
@@ -62,6 +63,17 @@ bool tensor_core(const rdvb_attention* a) {
     return rdvb_host::tensor_map_encoder() != nullptr;
 }
 
+// Whether the few-row kernel takes the forward pass: at most eight rows a key
+// head, rows of whole 16-byte pieces up to 128 dimensions, 16-byte aligned.
+bool few_rows(const rdvb_attention* a) {
+    const int vec = a->dtype == RDVB_F32 ? 4 : 8;
+    if (a->q_len * (a->heads / a->kv_heads) > kFewRows || a->dim > 128 || a->dim % vec) return false;
+    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (a->q_stride[i] % vec || a->k_stride[i] % vec || a->v_stride[i] % vec) return false;
+    return true;
+}
+
 // The map of [batch, length, heads, dim] that a tile of 128 positions of one
 // head is loaded by, in atoms of 64 dimensions; past the ends it reads 0.
 int encode(TcMap* out, const rdvb_attention* a, const void* base, const int64_t* stride, int64_t length, int heads) {
@@ -106,7 +118,7 @@ int splits_for(int64_t blocks, int64_t steps, int64_t slots, double step_us, dou
 }
 
 struct Plan {
-    bool tc;
+    bool tc, few;
     int forward, dq, dkv;  // splits
     int64_t forward_len, dq_len, dkv_len;
     int64_t forward_bytes, backward_bytes, delta_bytes, q_pad;
@@ -126,6 +138,14 @@ Plan plan(const rdvb_attention* a) {
     p.forward = splits_for((p.tc ? ceil_div(q_tiles, 2) : q_tiles) * a->heads * a->batch, k_tiles, slots,
                            p.tc ? 1.2 : 8.0, rows * row_bytes);
     p.forward_len = ceil_div(k_tiles, p.forward) * tile;
+    p.few = few_rows(a);
+    if (p.few) {
+        // three blocks a processor stream the keys, 64 or more each
+        const int64_t heads = static_cast<int64_t>(a->batch) * a->kv_heads;
+        const int64_t most = std::min<int64_t>(ceil_div(a->kv_len, 64), kMaxSplits);
+        const int64_t want = std::max<int64_t>(1, std::min(most, 3 * 148 / std::max<int64_t>(heads, 1)));
+        p.forward_len = ceil_div(ceil_div(a->kv_len, want), 64) * 64;
+    }
     p.forward = static_cast<int>(std::max<int64_t>(1, ceil_div(a->kv_len, std::max<int64_t>(p.forward_len, 1))));
     p.forward_bytes = p.forward > 1 ? round16(p.forward * rows * 8) + p.forward * rows * a->dim * 4 : 0;
     // gradients
@@ -216,6 +236,25 @@ int launch_tc_forward(const rdvb_attention* a, const Params& p, const rdvb_host:
                     : go(tc_forward_kernel<64, false>, TcForward<64>::kBytes);
     return bf16 ? go(tc_forward_kernel<128, true>, TcForward<128>::kBytes)
                 : go(tc_forward_kernel<128, false>, TcForward<128>::kBytes);
+}
+
+template <typename T>
+int launch_few(const rdvb_attention* a, const Params& p, cudaStream_t st) {
+    const int64_t blocks = static_cast<int64_t>(a->batch) * a->kv_heads * p.splits;
+    if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "few_kernel: too many blocks");
+    const int64_t rows = a->q_len * (a->heads / a->kv_heads), lanes = a->dim / static_cast<int>(16 / sizeof(T));
+    auto go = [&](auto n) {
+        constexpr int kLanes = decltype(n)::value;
+        const unsigned grid = static_cast<unsigned>(blocks);
+        if (rows <= 1) few_kernel<T, kLanes, 1><<<grid, kFewThreads, 0, st>>>(p);
+        else if (rows <= 2) few_kernel<T, kLanes, 2><<<grid, kFewThreads, 0, st>>>(p);
+        else if (rows <= 4) few_kernel<T, kLanes, 4><<<grid, kFewThreads, 0, st>>>(p);
+        else few_kernel<T, kLanes, 8><<<grid, kFewThreads, 0, st>>>(p);
+    };
+    if (lanes <= 8) go(std::integral_constant<int, 8>{});
+    else if (lanes <= 16) go(std::integral_constant<int, 16>{});
+    else if constexpr (sizeof(T) == 4) go(std::integral_constant<int, 32>{});
+    return rdvb_host::launched("few_kernel");
 }
 
 // dQ, dK and dV of a call that tensor_core() takes; `join` sums parts.
@@ -321,7 +360,12 @@ int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void*
     p.part_stat = static_cast<float*>(workspace);
     p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + round16(p.splits * rows * 8));
     const int64_t blocks = ceil_div(a->q_len, tile_of(a, l.tc)) * a->heads * a->batch * p.splits;
-    if (l.tc) {
+    if (l.few) {
+        const int rc = a->dtype == RDVB_F32   ? launch_few<float>(a, p, st)
+                       : a->dtype == RDVB_F16 ? launch_few<__half>(a, p, st)
+                                              : launch_few<__nv_bfloat16>(a, p, st);
+        if (rc) return rc;
+    } else if (l.tc) {
         if (int rc = launch_tc_forward(a, p, dev, st)) return rc;
     } else if (int rc = RDVB_BY_DIM(forward_kernel, kForwardBytes, blocks, )) {
         return rc;

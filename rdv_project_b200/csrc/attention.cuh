@@ -288,32 +288,60 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
     }
 }
 
-// Joins the splits of the forward pass in split order: a warp a row.
+constexpr int kMaxSplits = 128;
+
+// Joins the splits of the forward pass in split order: a warp a row, a lane
+// up to four splits' weights.
 __global__ void __launch_bounds__(kThreads) join_forward_kernel(const Params p) {
     const int64_t rows = static_cast<int64_t>(p.batch) * p.q_len * p.heads;
     const int64_t row = blockIdx.x * static_cast<int64_t>(kThreads / 32) + threadIdx.x / 32;
     if (row >= rows) return;
     const int lane = threadIdx.x % 32;
-    float top = -INFINITY;
+    constexpr int kMine = kMaxSplits / 32;
+    float top = -INFINITY, tops[kMine], totals[kMine];
     bool any = false;
-    for (int s = 0; s < p.splits; ++s) {
-        if (p.part_stat[2 * (s * rows + row) + 1] == -1.0f) continue;
-        any = true;
-        top = fmaxf(top, p.part_stat[2 * (s * rows + row)]);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int s = 32 * i + lane;
+        tops[i] = -INFINITY;
+        totals[i] = 0.0f;
+        if (s < p.splits) {
+            const float2 v = reinterpret_cast<const float2*>(p.part_stat)[s * rows + row];
+            if (v.y != -1.0f) {
+                any = true;
+                tops[i] = v.x;
+                totals[i] = v.y;
+            }
+        }
+        top = fmaxf(top, tops[i]);
     }
+    any = __any_sync(0xffffffffu, any);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
     float total = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float l = p.part_stat[2 * (s * rows + row) + 1];
-        if (l != -1.0f) total = fmaf(l, exp2f(p.part_stat[2 * (s * rows + row)] - base), total);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        tops[i] = exp2f(tops[i] - base);  // the split's weight
+        total = fmaf(totals[i], tops[i], total);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const float inv = 1.0f / total;
-    for (int d = lane; d < p.dim; d += 32) {
+    for (int d0 = 0; d0 < p.dim; d0 += 32) {
+        const int d = d0 + lane;
         float acc = 0.0f;
-        for (int s = 0; s < p.splits; ++s)
-            if (p.part_stat[2 * (s * rows + row) + 1] != -1.0f)
-                acc = fmaf(p.part[(s * rows + row) * p.dim + d], exp2f(p.part_stat[2 * (s * rows + row)] - base), acc);
-        store1(p.o, p.dtype, row * p.dim + d, any ? acc * inv : 0.0f);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int n = min(32, p.splits - 32 * i);
+#pragma unroll 4
+            for (int s = 0; s < n; ++s) {
+                const float f = __shfl_sync(0xffffffffu, tops[i], s);
+                // a split without an allowed key has weight 0 and wrote zeros
+                if (d < p.dim) acc = fmaf(p.part[((32 * i + s) * rows + row) * p.dim + d], f, acc);
+            }
+        }
+        if (d < p.dim) store1(p.o, p.dtype, row * p.dim + d, any ? acc * inv : 0.0f);
     }
     if (lane == 0 && p.lse) {
         const int64_t h = row % p.heads, q = row / p.heads % p.q_len, b = row / p.heads / p.q_len;

@@ -27,7 +27,7 @@ SOURCES = {
     "norm.cu": ["host.h", "types.cuh", "norm.cuh"],
     "dropout.cu": ["host.h", "types.cuh", "dropout.cuh"],
     "attention.cu": ["host.h", "types.cuh", "ptx.cuh", "attention.cuh", "attention_tc.cuh",
-                     "attention_tc_grad.cuh"],
+                     "attention_tc_grad.cuh", "attention_few.cuh"],
 }
 
 
