@@ -24,7 +24,6 @@ current stream, with workspaces from torch's allocator.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -39,19 +38,18 @@ _ACTIVATIONS = {None: N.RDVB_ACT_NONE, "relu": N.RDVB_ACT_RELU, "silu": N.RDVB_A
 
 def _tensor(x) -> torch.Tensor:
     """x on the current device (a CUDA tensor that is there is aliased)."""
-    if isinstance(x, torch.Tensor) and x.is_cuda and x.device.index == torch.cuda.current_device():
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() == torch.cuda.current_device():
         return x
     current_device()
     return as_device_tensor(x)
 
 
-def _need(ok, text) -> None:
-    if not ok:
-        raise ValueError(text)
-
-
 def _workspace(nbytes: int, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _dense_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _ptr(t):
@@ -59,32 +57,41 @@ def _ptr(t):
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            return True
+    return False
 
 
 # ---------------------------------------------------------------- group norm
 
 
+def _channel_param(name, p, c):
+    if p is None:
+        return None
+    p = _tensor(p)
+    if p.dim() != 1 or p.shape[0] != c or p.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be [{c}] of float32, float16 or bfloat16, got {tuple(p.shape)} of {p.dtype}")
+    return p.contiguous()
+
+
 def _norm_args(x, groups, weight, bias, activation):
     x = _tensor(x).contiguous()
-    _need(x.dim() >= 2, f"x must be [N, ..., C], got {tuple(x.shape)}")
-    _need(x.dtype in _DTYPES, f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    if not (x.dim() >= 2):
+        raise ValueError(f"x must be [N, ..., C], got {tuple(x.shape)}")
+    if not (x.dtype in _DTYPES):
+        raise ValueError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
     c = x.shape[-1]
-    _need(c > 0 and isinstance(groups, int) and groups > 0 and c % groups == 0,
-          f"groups ({groups}) must be a whole number that divides the channels ({c})")
-    _need(activation in _ACTIVATIONS, f"activation must be None, 'relu', 'silu' or 'gelu', got {activation!r}")
-    params = []
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None:
-            p = _tensor(p)
-            _need(tuple(p.shape) == (c,) and p.dtype in _DTYPES,
-                  f"{name} must be [{c}] of float32, float16 or bfloat16, got {tuple(p.shape)} of {p.dtype}")
-            p = p.contiguous()
-        params.append(p)
-    w, b = params
+    if not (c > 0 and isinstance(groups, int) and groups > 0 and c % groups == 0):
+        raise ValueError(f"groups ({groups}) must be a whole number that divides the channels ({c})")
+    if not (activation in _ACTIVATIONS):
+        raise ValueError(f"activation must be None, 'relu', 'silu' or 'gelu', got {activation!r}")
+    w, b = _channel_param("weight", weight, c), _channel_param("bias", bias, c)
     if w is not None and b is not None and w.dtype != b.dtype:
         w, b = w.float(), b.float()
-    kind = next((_DTYPES[p.dtype] for p in (w, b) if p is not None), N.RDVB_F32)
+    kind = N.RDVB_F32 if w is None and b is None else _DTYPES[b.dtype if w is None else w.dtype]
     return x, w, b, kind, x.shape[0], math.prod(x.shape[1:-1]), c
 
 
@@ -117,10 +124,11 @@ def group_norm_backward(dy, x, stats, groups: int, weight=None, bias=None, activ
     a parameter that is None."""
     x, w, b, kind, n, rows, c = _norm_args(x, groups, weight, bias, activation)
     dy = _tensor(dy).contiguous()
-    _need(dy.shape == x.shape and dy.dtype == x.dtype, "dy must have x's shape and type")
+    if not (dy.shape == x.shape and dy.dtype == x.dtype):
+        raise ValueError("dy must have x's shape and type")
     stats = _tensor(stats).contiguous()
-    _need(tuple(stats.shape) == (n, groups, 2) and stats.dtype == torch.float32,
-          f"stats must be float32 [{n}, {groups}, 2]")
+    if not (tuple(stats.shape) == (n, groups, 2) and stats.dtype == torch.float32):
+        raise ValueError(f"stats must be float32 [{n}, {groups}, 2]")
     lib = N.lib()
     dx = torch.empty_like(x)
     dw = torch.empty(c, dtype=torch.float32, device=x.device) if w is not None else None
@@ -166,37 +174,44 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, activa
 
 def _states(name, t):
     t = _tensor(t)
-    _need(t.dim() == 4, f"{name} must be [batch, positions, heads, D], got {tuple(t.shape)}")
-    _need(t.dtype in _DTYPES, f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if not (t.dim() == 4):
+        raise ValueError(f"{name} must be [batch, positions, heads, D], got {tuple(t.shape)}")
+    if not (t.dtype in _DTYPES):
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
 def _describe(q, k, v, lengths, mask, scale):
-    """The rdvb_attention of a call, and the tensors that it points into."""
+    """The rdvb_attention of a call, as bytes, and the tensors that it points into."""
     q, k, v = _states("q", q), _states("k", k), _states("v", v)
     b, lq, heads, d = q.shape
     lk, kv_heads = k.shape[1], k.shape[2]
-    _need(k.shape == v.shape, f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    _need(k.shape[0] == b and k.shape[3] == d, f"k and v must be [{b}, Lk, kv_heads, {d}], got {tuple(k.shape)}")
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must have one type")
-    _need(kv_heads > 0 and heads > 0 and heads % kv_heads == 0,
-          f"k's heads ({kv_heads}) must divide q's ({heads})")
+    if not (k.shape == v.shape):
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if not (k.shape[0] == b and k.shape[3] == d):
+        raise ValueError(f"k and v must be [{b}, Lk, kv_heads, {d}], got {tuple(k.shape)}")
+    if not (k.dtype == q.dtype and v.dtype == q.dtype):
+        raise ValueError("q, k and v must have one type")
+    if not (kv_heads > 0 and heads > 0 and heads % kv_heads == 0):
+        raise ValueError(f"k's heads ({kv_heads}) must divide q's ({heads})")
     if lengths is not None:
         lengths = _tensor(lengths)
-        _need(tuple(lengths.shape) == (b,) and not lengths.is_floating_point() and lengths.dtype != torch.bool,
-              f"lengths must be whole numbers [{b}]")
+        if not (tuple(lengths.shape) == (b,) and not lengths.is_floating_point() and lengths.dtype != torch.bool):
+            raise ValueError(f"lengths must be whole numbers [{b}]")
         if lengths.dtype != torch.int32:
             lengths = lengths.clamp(0, lk).to(torch.int32)
         lengths = lengths.contiguous()
     if mask is not None:
         mask = _tensor(mask)
-        _need(tuple(mask.shape) == (b, lk) and mask.dtype == torch.bool, f"mask must be bool [{b}, {lk}]")
+        if not (tuple(mask.shape) == (b, lk) and mask.dtype == torch.bool):
+            raise ValueError(f"mask must be bool [{b}, {lk}]")
         mask = mask if mask.stride(1) == 1 or lk <= 1 else mask.contiguous()
-    a = N.Attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), _ptr(mask), 0 if mask is None else mask.stride(0),
-        q.stride()[:3], k.stride()[:3], v.stride()[:3], lq, lk, _DTYPES[q.dtype], b, heads, kv_heads, d,
+    packed = N.ATTENTION_PACK(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+        0 if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0),
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], lq, lk, _DTYPES[q.dtype], b, heads, kv_heads, d,
         d ** -0.5 if scale is None else float(scale))
-    return a, (q, k, v, lengths, mask)
+    return packed, (q, k, v, lengths, mask)
 
 
 def _dense16(t):
@@ -209,12 +224,12 @@ def _cross_attention(q, k, v, lengths, mask, scale, want_lse):
     a, held = _describe(q, k, v, lengths, mask, scale)
     q = held[0]
     lib = N.lib()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((a.batch, a.heads, a.q_len), dtype=torch.float32, device=q.device) if want_lse else None
-    nbytes = lib.rdvb_attention_workspace_bytes(ctypes.byref(a), 0)
+    out = _dense_like(q)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if want_lse else None
+    nbytes = lib.rdvb_attention_workspace_bytes(a, 0)
     ws = _workspace(nbytes, q.device)
     with _timed():
-        N.check(lib.rdvb_attention_forward(ctypes.byref(a), out.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
+        N.check(lib.rdvb_attention_forward(a, out.data_ptr(), _ptr(lse), _ptr(ws), nbytes,
                                            stream_handle()), "rdvb_attention_forward")
     return out, lse
 
@@ -234,17 +249,18 @@ def cross_attention_backward(dout, q, k, v, out, lse, lengths=None, mask=None, s
     q, k = held[0], held[1]
     dout, out, lse = _dense16(dout), _dense16(out), _tensor(lse).contiguous()
     for name, t in (("dout", dout), ("out", out)):
-        _need(t.shape == q.shape and t.dtype == q.dtype, f"{name} must have q's shape and type")
-    _need(tuple(lse.shape) == (a.batch, a.heads, a.q_len) and lse.dtype == torch.float32,
-          f"lse must be float32 [{a.batch}, {a.heads}, {a.q_len}]")
+        if not (t.shape == q.shape and t.dtype == q.dtype):
+            raise ValueError(f"{name} must have q's shape and type")
+    b, lq, heads = q.shape[:3]
+    if not (tuple(lse.shape) == (b, heads, lq) and lse.dtype == torch.float32):
+        raise ValueError(f"lse must be float32 [{b}, {heads}, {lq}]")
     lib = N.lib()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    nbytes = lib.rdvb_attention_workspace_bytes(ctypes.byref(a), 1)
+    dq, dk, dv = _dense_like(q), _dense_like(k), _dense_like(k)
+    nbytes = lib.rdvb_attention_workspace_bytes(a, 1)
     ws = _workspace(nbytes, q.device)
     with _timed():
         N.check(lib.rdvb_attention_backward(
-            ctypes.byref(a), dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            a, dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), _ptr(ws), nbytes, stream_handle()), "rdvb_attention_backward")
     return dq, dk, dv
 
@@ -284,15 +300,19 @@ def cross_attention(q, k, v, lengths=None, mask=None, scale=None) -> torch.Tenso
 
 def _dropout(x, p, seed, offset, residual):
     x = _tensor(x).contiguous()
-    _need(x.dtype in _DTYPES, f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    if not (x.dtype in _DTYPES):
+        raise ValueError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
     p = float(p)
-    _need(0.0 <= p and round(min(p, 2.0) * 2 ** 32) < 2 ** 32, f"p must be in [0, 1 - 2**-32), got {p}")
-    _need(isinstance(seed, int) and 0 <= seed < 2 ** 64, "seed must be a whole number in [0, 2**64)")
-    _need(isinstance(offset, int) and 0 <= offset and offset + (x.numel() + 3) // 4 <= 2 ** 64,
-          "offset must be a whole number >= 0 whose counters fit 64 bits")
+    if not (0.0 <= p and round(min(p, 2.0) * 2 ** 32) < 2 ** 32):
+        raise ValueError(f"p must be in [0, 1 - 2**-32), got {p}")
+    if not (isinstance(seed, int) and 0 <= seed < 2 ** 64):
+        raise ValueError("seed must be a whole number in [0, 2**64)")
+    if not (isinstance(offset, int) and 0 <= offset and offset + (x.numel() + 3) // 4 <= 2 ** 64):
+        raise ValueError("offset must be a whole number >= 0 whose counters fit 64 bits")
     if residual is not None:
         residual = _tensor(residual).contiguous()
-        _need(residual.shape == x.shape and residual.dtype == x.dtype, "residual must have x's shape and type")
+        if not (residual.shape == x.shape and residual.dtype == x.dtype):
+            raise ValueError("residual must have x's shape and type")
     y = torch.empty_like(x)
     with _timed():
         N.check(N.lib().rdvb_dropout(x.data_ptr(), _ptr(residual), y.data_ptr(), _DTYPES[x.dtype], x.numel(), p, seed,
@@ -392,7 +412,7 @@ class CrossAttentionTensorOp(TensorOperation):
         a, _ = _describe(q.view(1, q.shape[0], self.heads, -1), k.view(1, k.shape[0], self.kv_heads, -1),
                          v.view(1, v.shape[0], self.kv_heads, -1), None, None, self.scale)
         lib = N.lib()
-        nbytes = lib.rdvb_attention_workspace_bytes(ctypes.byref(a), 0)
+        nbytes = lib.rdvb_attention_workspace_bytes(a, 0)
         ws = _workspace(nbytes, q.device)
-        N.check(lib.rdvb_attention_forward(ctypes.byref(a), self._result._tensor.data_ptr(), None, _ptr(ws), nbytes,
+        N.check(lib.rdvb_attention_forward(a, self._result._tensor.data_ptr(), None, _ptr(ws), nbytes,
                                            stream_handle()), "rdvb_attention_forward")

@@ -41,14 +41,7 @@ def profiling_submit_times() -> float:
 
 
 @contextlib.contextmanager
-def _timed():
-    """Context around one operator's launches: with profiling on, records CUDA
-    events on the current stream and adds the elapsed seconds to the
-    submit-time total (synchronizing on the end event, like the reference's
-    blocking submit)."""
-    if not __PROFILING__:
-        yield
-        return
+def _timed_events():
     global __submit_times__
     s = torch.cuda.current_stream()
     start = torch.cuda.Event(enable_timing=True)
@@ -58,6 +51,17 @@ def _timed():
     end.record(s)
     end.synchronize()
     __submit_times__ += start.elapsed_time(end) / 1000.0
+
+
+_UNTIMED = contextlib.nullcontext()
+
+
+def _timed():
+    """Context around one operator's launches: with profiling on, records CUDA
+    events on the current stream and adds the elapsed seconds to the
+    submit-time total (synchronizing on the end event, like the reference's
+    blocking submit)."""
+    return _timed_events() if __PROFILING__ else _UNTIMED
 
 
 def current_device() -> torch.device:

@@ -323,3 +323,45 @@ def test_multicast_copy_validation(lib):
     rc = lib.rdvb_multicast_copy(None, 0, 32, 16, None)
     assert rc == -1 and "NULL" in N.last_error()
     assert lib.rdvb_multicast_copy(None, 0, 0, 16, None) == 0
+
+
+def test_block_operators_validation_before_any_device_work(lib):
+    """rdvb_group_norm*, rdvb_attention_*, rdvb_dropout: descriptions and sizes
+    are checked, and calls with nothing to do return, without a device."""
+    import rdv_project_b200._native as N
+
+    def norm(dtype=0, n=1, rows=4, c=8, groups=2, kind=0, act=0, eps=1e-5):
+        return lib.rdvb_group_norm(None, dtype, n, rows, c, groups, None, None, kind, act, eps, None, None, None, 0, None)
+
+    for kw, word in (({"dtype": 5}, "dtype"), ({"kind": 3}, "param_dtype"), ({"groups": 3}, "groups"),
+                     ({"groups": 0}, "groups"), ({"act": 4}, "activation"), ({"eps": float("nan")}, "eps"),
+                     ({"n": -1}, ">= 0"), ({}, "NULL")):
+        assert norm(**kw) == -1 and word in N.last_error()
+    assert norm(n=0) == 0 and norm(rows=0) == 0
+    assert lib.rdvb_group_norm_workspace_bytes(2, 100, 64, 8, 1) > lib.rdvb_group_norm_workspace_bytes(2, 100, 64, 8, 0)
+
+    def attention(**kw):
+        a = N.Attention(dtype=1, batch=1, heads=4, kv_heads=2, dim=64, q_len=3, kv_len=5, scale=0.125)
+        for name, value in kw.items():
+            setattr(a, name, value)
+        return lib.rdvb_attention_forward(ctypes.byref(a), None, None, None, 0, None)
+
+    for kw, word in (({"dtype": 7}, "dtype"), ({"kv_heads": 3}, "kv_heads"), ({"scale": float("inf")}, "scale"),
+                     ({"q_len": -1}, ">= 0"), ({}, "NULL")):
+        assert attention(**kw) == -1 and word in N.last_error()
+    assert attention(dim=257) == -2 and "dimension" in N.last_error()
+    assert attention(batch=0) == 0 and attention(q_len=0) == 0
+    assert lib.rdvb_attention_forward(None, None, None, None, 0, None) == -1
+    for kw, word in (({"p": 1.0}, "p must"), ({"p": -0.5}, "p must"), ({"p": float("nan")}, "p must"), ({"n": -1}, "n must"),
+                     ({}, "NULL")):
+        args = {"n": 4, "p": 0.5, **kw}
+        assert lib.rdvb_dropout(None, None, None, 0, args["n"], args["p"], 0, 0, None) == -1 and word in N.last_error()
+    assert lib.rdvb_dropout(None, None, None, 0, 0, 0.5, 0, 0, None) == 0
+
+
+def test_attention_description_bytes():
+    import rdv_project_b200._native as N
+
+    values = [11, 12, 13, 14, 15, 16, *range(20, 29), 30, 31, 1, 2, 4, 2, 64, 0.125]
+    a = N.Attention(*values[:6], tuple(values[6:9]), tuple(values[9:12]), tuple(values[12:15]), *values[15:])
+    assert bytes(a) == N.ATTENTION_PACK(*values)
