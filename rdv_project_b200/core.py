@@ -70,7 +70,14 @@ def current_device() -> torch.device:
     return torch.device("cuda", torch.cuda.current_device())
 
 
+# torch's own getter of the current stream's handle, without building a Stream
+# object around it (0.1 us instead of 3); absent from builds without CUDA.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle() -> int:
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 

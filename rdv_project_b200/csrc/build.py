@@ -24,7 +24,7 @@ SOURCES = {
     "rdvb.cu": ["host.h", "ptx.cuh", "rng.cuh", "mlp_tc.cuh", "mlp_simt.cuh", "winograd.cuh", "winograd_f43.cuh",
                 "raymarch.cuh", "transmittance.cuh", "resample.cuh", "conv_tc.cuh", "sampler.cuh", "pbvr.cuh",
                 "exchange.cuh"],
-    "norm.cu": ["host.h", "types.cuh", "norm.cuh"],
+    "norm.cu": ["host.h", "types.cuh", "ptx.cuh", "norm.cuh"],
     "dropout.cu": ["host.h", "types.cuh", "dropout.cuh"],
     "attention.cu": ["host.h", "types.cuh", "ptx.cuh", "attention.cuh", "attention_tc.cuh",
                      "attention_tc_grad.cuh", "attention_few.cuh"],

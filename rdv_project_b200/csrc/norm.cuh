@@ -6,11 +6,16 @@
 //   dx = rstd (w dz - mean(w dz) - xhat mean(w dz xhat)).
 //
 // Bound: memory; ~10 (forward) and ~25 (backward) float32 operations an
-// element. A pass over the data takes sums of a slab of rows (a block a
-// slab; threads lie along the channels, 16 bytes each, so a warp reads whole
-// lines whatever the group's width), a second pass joins the slabs' sums
-// in slab order -- no atomics, so results repeat bit for bit -- and
-// normalises. The second pass finds what fits in L2 there.
+// element, two of them of the exponential unit for silu. A pass over the data
+// takes sums of a slab of rows (a block a slab; threads lie along the
+// channels, up to 16 bytes each, so a warp reads whole lines whatever the
+// group's width), a second pass joins the slabs' sums in slab order -- no
+// atomics, so results repeat bit for bit -- and normalises. The second pass
+// finds what fits in L2 there. (One launch that kept the slabs in shared
+// memory and waited for the sample's other blocks read less, but the waits and
+// the joins by every block cost more: 125 us for 8 x 256 x 256 x 64 float16.)
+// A sample that fits one block's shared memory takes one launch
+// (small_kernel).
 //
 // A thread sums its elements' distances from its first one in float32, so a
 // mean far from zero costs no digits; parts are joined by their means, in 64
@@ -19,6 +24,8 @@
 #pragma once
 #include <cstdint>
 
+#define RDVB_STATUS_ELSEWHERE
+#include "ptx.cuh"
 #include "types.cuh"
 
 namespace rdvb {
@@ -28,6 +35,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxGroups = 2048;
 constexpr int kMaxSlabs = 128;
+constexpr int kRuntime = -1;  // a kernel's activation is Params::act
 
 enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
@@ -58,7 +66,9 @@ __device__ __forceinline__ float param_at(const void* p, int type, int i, float 
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
+// Two exponential-unit instructions; both are within 2 units in the last
+// place, so the result is within about 4.
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
 
 __device__ __forceinline__ float activate(float z, int act) {
     if (act == kRelu) return z < 0.0f ? 0.0f : z;  // keeps a NaN
@@ -84,22 +94,6 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// A block's place: sample, slab, and how its threads lie over `tile` of the
-// channel vectors (cols of them) and `lanes` rows at a time.
-struct Place {
-    int sample, slab;
-    int64_t row0, rows;
-};
-
-__device__ __forceinline__ Place place(const Params& p) {
-    Place a;
-    a.sample = blockIdx.x / p.slabs;
-    a.slab = blockIdx.x % p.slabs;
-    a.row0 = a.slab * p.slab_rows;
-    const int64_t left = p.rows - a.row0;
-    a.rows = left < p.slab_rows ? left : p.slab_rows;
-    return a;
-}
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -107,72 +101,106 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
+template <int kAct>
+__device__ __forceinline__ int act_of(const Params& p) {
+    return kAct == kRuntime ? p.act : kAct;
+}
+
+// A block's sample and slab.
+struct Place {
+    int sample, slab, rows;
+    int64_t start;  // its first element
+};
+__device__ __forceinline__ Place place(const Params& p) {
+    Place a;
+    a.sample = blockIdx.x / p.slabs;
+    a.slab = blockIdx.x % p.slabs;
+    const int64_t row0 = a.slab * p.slab_rows, left = p.rows - row0;
+    a.rows = static_cast<int>(left < p.slab_rows ? left : p.slab_rows);
+    a.start = (a.sample * p.rows + row0) * p.c;
+    return a;
+}
+
+// e / d of small whole numbers from the float32 reciprocal of d.
+__device__ __forceinline__ int quotient(int e, float inv) { return static_cast<int>((e + 0.5f) * inv); }
+
+// kOne: a thread's vector lies in one group, so its statistics are one
+// number; otherwise each of its channels has its own.
+
 // Slab sums of the forward pass: mean_part[sample][slab][group]. Dynamic
 // shared memory: a double and a float a group.
-template <typename T, int kVec>
+template <typename T, int kVec, bool kOne>
 __global__ void __launch_bounds__(kThreads) sums_kernel(const Params p) {
-    __shared__ double s_mean[kVec * kThreads];
-    __shared__ float s_dev[kVec * kThreads];
+    constexpr int kStat = kOne ? 1 : kVec;
+    __shared__ double s_mean[kStat * kThreads];
+    __shared__ float s_dev[kStat * kThreads];
     extern __shared__ double s_join[];  // means, then (float) squared deviations
     float* s_join_dev = reinterpret_cast<float*>(s_join + p.groups);
     const Place a = place(p);
-    const int cols = p.c / kVec;
+    const int cols = p.c / kVec, cells = kOne ? p.per / kVec : p.per;  // cells of a group in a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const T* base = static_cast<const T*>(p.x) + (a.sample * p.rows + a.row0) * p.c;
     for (int col0 = 0; col0 < cols; col0 += kThreads) {
         const int tile = min(cols - col0, kThreads);
         const int lanes = kThreads / tile;
         const int tx = threadIdx.x % tile, ty = threadIdx.x / tile;
-        const int64_t mine = ty < lanes && ty < a.rows ? (a.rows - ty + lanes - 1) / lanes : 0;
-        float first[kVec], s1[kVec] = {}, s2[kVec] = {};
+        const int mine = ty < lanes && ty < a.rows ? (a.rows - ty + lanes - 1) / lanes : 0;
+        float first[kStat] = {}, s1[kStat] = {}, s2[kStat] = {};
         if (mine > 0) {
-            const T* at = base + static_cast<int64_t>(ty) * p.c + static_cast<int64_t>(col0 + tx) * kVec;
+            const T* at = static_cast<const T*>(p.x) + a.start + static_cast<int64_t>(ty) * p.c + (col0 + tx) * kVec;
             const int64_t step = static_cast<int64_t>(lanes) * p.c;
-            load_f32<T, kVec>(at, first);
-#pragma unroll 4
-            for (int64_t r = 1; r < mine; ++r) {
+            {
                 float v[kVec];
-                load_f32<T, kVec>(at + r * step, v);
+                load_f32<T, kVec>(at, v);
+#pragma unroll
+                for (int i = 0; i < kStat; ++i) first[i] = v[i];
+            }
+#pragma unroll 8
+            for (int r = 0; r < mine; ++r, at += step) {
+                float v[kVec];
+                load_f32<T, kVec>(at, v);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
-                    const float d = v[i] - first[i];
-                    s1[i] += d;
-                    s2[i] = fmaf(d, d, s2[i]);
+                    const int k = kOne ? 0 : i;
+                    const float d = v[i] - first[k];
+                    s1[k] += d;
+                    s2[k] = fmaf(d, d, s2[k]);
                 }
             }
         }
-        const float inv = mine > 0 ? 1.0f / static_cast<float>(mine) : 0.0f;
+        const float inv = mine > 0 ? 1.0f / static_cast<float>(mine * (kVec / kStat)) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            s_mean[i * kThreads + threadIdx.x] = mine > 0 ? static_cast<double>(first[i]) + s1[i] * inv : 0.0;
+        for (int i = 0; i < kStat; ++i) {
+            s_mean[i * kThreads + threadIdx.x] = static_cast<double>(first[i]) + s1[i] * inv;
             s_dev[i * kThreads + threadIdx.x] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f) + 0.0f * s2[i];
         }
         __syncthreads();
-        // a warp a group: its channels inside this tile, over the thread rows
-        const int c0 = col0 * kVec, c1 = c0 + tile * kVec;
-        const int used = a.rows < lanes ? static_cast<int>(a.rows) : lanes;
-        for (int g = c0 / p.per + warp; g < p.groups && g * p.per < c1; g += kWarps) {
-            const int lo = max(g * p.per, c0), width = min((g + 1) * p.per, c1) - lo;
+        // a warp a group: its cells inside this tile, over the thread rows
+        const int c0 = col0 * kStat, c1 = c0 + tile * kStat;
+        const int used = min(a.rows, lanes);
+        for (int g = c0 / cells + warp; g < p.groups && g * cells < c1; g += kWarps) {
+            const int lo = max(g * cells, c0), width = min((g + 1) * cells, c1) - lo;
+            const float inv_width = 1.0f / static_cast<float>(width);
             double total = 0.0;
             for (int e = lane; e < width * used; e += 32) {
-                const int ch = lo - c0 + e % width, row = e / width;
-                const double m = static_cast<double>((a.rows - row + lanes - 1) / lanes);
-                total += m * s_mean[(ch % kVec) * kThreads + row * tile + ch / kVec];
+                const int row = quotient(e, inv_width), cell = lo - c0 + e - row * width;
+                total += static_cast<double>((a.rows - row + lanes - 1) / lanes) *
+                         s_mean[(cell % kStat) * kThreads + row * tile + cell / kStat];
             }
-            const double count = static_cast<double>(a.rows) * width;
-            const double mean = warp_sum(total) / count;
+            const double cell_rows = static_cast<double>(a.rows) * width;
+            const double mean = warp_sum(total) / cell_rows;
             float dev = 0.0f;
             for (int e = lane; e < width * used; e += 32) {
-                const int ch = lo - c0 + e % width, row = e / width;
-                const float m = static_cast<float>((a.rows - row + lanes - 1) / lanes);
-                const int at = (ch % kVec) * kThreads + row * tile + ch / kVec;
+                const int row = quotient(e, inv_width), cell = lo - c0 + e - row * width;
+                const int at = (cell % kStat) * kThreads + row * tile + cell / kStat;
+                const float m = static_cast<float>((a.rows - row + lanes - 1) / lanes * (kVec / kStat));
                 const float d = static_cast<float>(s_mean[at] - mean);
                 dev += s_dev[at] + m * d * d;
             }
             dev = warp_sum(dev);
             if (lane == 0) {
-                // with the channels of this group that an earlier tile has summed
-                const double before = static_cast<double>(a.rows) * (lo - g * p.per);
+                // with the cells of this group that an earlier tile has summed
+                const double count = cell_rows * (kVec / kStat);
+                const double before = static_cast<double>(a.rows) * (lo - g * cells) * (kVec / kStat);
                 if (before == 0.0) {
                     s_join[g] = mean;
                     s_join_dev[g] = dev;
@@ -215,8 +243,9 @@ __device__ __forceinline__ void join_slabs(const Params& p, int sample, float* s
 }
 
 // Second pass of the forward pass. Dynamic shared memory: 2 groups floats.
-template <typename T, int kVec>
+template <typename T, int kVec, bool kOne, int kAct>
 __global__ void __launch_bounds__(kThreads) apply_kernel(const Params p) {
+    constexpr int kStat = kOne ? 1 : kVec;
     extern __shared__ float s_group[];
     const Place a = place(p);
     join_slabs(p, a.sample, s_group);
@@ -229,45 +258,71 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const Params p) {
         }
     }
     const int cols = p.c / kVec;
-    const int64_t start = (a.sample * p.rows + a.row0) * p.c;
     for (int col0 = 0; col0 < cols; col0 += kThreads) {
         const int tile = min(cols - col0, kThreads);
         const int lanes = kThreads / tile;
         const int tx = threadIdx.x % tile, ty = threadIdx.x / tile;
         if (ty >= lanes) continue;
         const int c0 = (col0 + tx) * kVec;
-        float mean[kVec], gain[kVec], bias[kVec];
+        float mean[kStat], gain[kVec], bias[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
             const int g = (c0 + i) / p.per;
-            mean[i] = s_group[g];
+            if (i < kStat) mean[i] = s_group[g];
             gain[i] = s_group[p.groups + g] * param_at(p.weight, p.param_type, c0 + i, 1.0f);
             bias[i] = param_at(p.bias, p.param_type, c0 + i, 0.0f);
         }
-        const T* in = static_cast<const T*>(p.x) + start + c0;
-        T* out = static_cast<T*>(p.out) + start + c0;
+        const int64_t first = a.start + static_cast<int64_t>(ty) * p.c + c0, step = static_cast<int64_t>(lanes) * p.c;
+        const T* in = static_cast<const T*>(p.x) + first;
+        T* out = static_cast<T*>(p.out) + first;
 #pragma unroll 4
-        for (int64_t r = ty; r < a.rows; r += lanes) {
+        for (int r = ty; r < a.rows; r += lanes, in += step, out += step) {
             float v[kVec];
-            load_f32<T, kVec>(in + r * p.c, v);
+            load_f32<T, kVec>(in, v);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(v[i] - mean[i], gain[i], bias[i]), p.act);
-            store_f32<T, kVec>(out + r * p.c, v);
+            for (int i = 0; i < kVec; ++i)
+                v[i] = activate(fmaf(v[i] - mean[kOne ? 0 : i], gain[i], bias[i]), act_of<kAct>(p));
+            store_f32<T, kVec>(out, v);
         }
     }
 }
 
+// A thread's channels of a backward pass: their group's statistics and their
+// own parameters.
+template <int kVec, bool kOne>
+struct Channels {
+    static constexpr int kStat = kOne ? 1 : kVec;
+    float mean[kStat], rstd[kStat], w[kVec], bias[kVec];
+    __device__ __forceinline__ void load(const Params& p, int sample, int c0) {
+        const float* stats = p.stats + static_cast<int64_t>(sample) * p.groups * 2;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            if (i < kStat) {
+                const int g = (c0 + i) / p.per;
+                mean[i] = stats[2 * g];
+                rstd[i] = stats[2 * g + 1];
+            }
+            w[i] = param_at(p.weight, p.param_type, c0 + i, 1.0f);
+            bias[i] = param_at(p.bias, p.param_type, c0 + i, 0.0f);
+        }
+    }
+    // xhat and dz of channel i
+    template <int kAct>
+    __device__ __forceinline__ float2 at(const Params& p, int i, float x, float dy) const {
+        const int k = kOne ? 0 : i;
+        const float xhat = (x - mean[k]) * rstd[k];
+        return make_float2(xhat, dy * slope(fmaf(xhat, w[i], bias[i]), act_of<kAct>(p)));
+    }
+};
+
 // Slab sums of the backward pass: chan_part[sample][slab][channel] and
 // group_part[sample][slab][group].
-template <typename T, int kVec>
+template <typename T, int kVec, bool kOne, int kAct>
 __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const Params p) {
     __shared__ float s_dz[kVec * kThreads], s_dzx[kVec * kThreads];
-    extern __shared__ float s_group[];  // sums of w dz, then of w dz xhat
     const Place a = place(p);
     const int cols = p.c / kVec;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t start = (a.sample * p.rows + a.row0) * p.c;
-    const float* stats = p.stats + static_cast<int64_t>(a.sample) * p.groups * 2;
     float2* chan = p.chan_part + static_cast<int64_t>(blockIdx.x) * p.c;
     for (int col0 = 0; col0 < cols; col0 += kThreads) {
         const int tile = min(cols - col0, kThreads);
@@ -276,28 +331,21 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const Params p) {
         float sdz[kVec] = {}, sdzx[kVec] = {};
         if (ty < lanes) {
             const int c0 = (col0 + tx) * kVec;
-            float mean[kVec], rstd[kVec], w[kVec], bias[kVec];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const int g = (c0 + i) / p.per;
-                mean[i] = stats[2 * g];
-                rstd[i] = stats[2 * g + 1];
-                w[i] = param_at(p.weight, p.param_type, c0 + i, 1.0f);
-                bias[i] = param_at(p.bias, p.param_type, c0 + i, 0.0f);
-            }
-            const T* x = static_cast<const T*>(p.x) + start + c0;
-            const T* dy = static_cast<const T*>(p.dy) + start + c0;
+            Channels<kVec, kOne> ch;
+            ch.load(p, a.sample, c0);
+            const int64_t first = a.start + static_cast<int64_t>(ty) * p.c + c0, step = static_cast<int64_t>(lanes) * p.c;
+            const T* x = static_cast<const T*>(p.x) + first;
+            const T* dy = static_cast<const T*>(p.dy) + first;
 #pragma unroll 2
-            for (int64_t r = ty; r < a.rows; r += lanes) {
+            for (int r = ty; r < a.rows; r += lanes, x += step, dy += step) {
                 float v[kVec], d[kVec];
-                load_f32<T, kVec>(x + r * p.c, v);
-                load_f32<T, kVec>(dy + r * p.c, d);
+                load_f32<T, kVec>(x, v);
+                load_f32<T, kVec>(dy, d);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
-                    const float xhat = (v[i] - mean[i]) * rstd[i];
-                    const float dz = d[i] * slope(fmaf(xhat, w[i], bias[i]), p.act);
-                    sdz[i] += dz;
-                    sdzx[i] = fmaf(dz, xhat, sdzx[i]);
+                    const float2 g = ch.template at<kAct>(p, i, v[i], d[i]);
+                    sdz[i] += g.y;
+                    sdzx[i] = fmaf(g.y, g.x, sdzx[i]);
                 }
             }
         }
@@ -323,7 +371,6 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const Params p) {
                 sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 sumx += __shfl_xor_sync(0xffffffffu, sumx, o);
             }
-            __syncwarp();
             if (ch < width && (e & 3) == 0) chan[col0 * kVec + ch] = make_float2(sum, sumx);
         }
         __syncthreads();  // also makes this block's chan entries readable below
@@ -343,33 +390,43 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const Params p) {
     }
 }
 
+// The channel gradients of 32 channels from `parts` rows of chan_part, in
+// order: warps over the parts, then over the warps.
+__device__ __forceinline__ void join_channels(const Params& p, int64_t parts, int ch0) {
+    __shared__ float2 s_part[kWarps][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ch = ch0 + lane;
+    float sum = 0.0f, sumx = 0.0f;
+    if (ch < p.c) {
+#pragma unroll 4
+        for (int64_t i = warp; i < parts; i += kWarps) {
+            const float2 v = p.chan_part[i * p.c + ch];
+            sum += v.x;
+            sumx += v.y;
+        }
+    }
+    s_part[warp][lane] = make_float2(sum, sumx);
+    __syncthreads();
+    if (warp == 0 && ch < p.c) {
+        for (int i = 1; i < kWarps; ++i) {
+            sum += s_part[i][lane].x;
+            sumx += s_part[i][lane].y;
+        }
+        if (p.dbias) p.dbias[ch] = sum;
+        if (p.dweight) p.dweight[ch] = sumx;
+    }
+}
+
 // Second pass of the backward pass: dx, and in the blocks past n * slabs the
-// channel gradients (32 channels a block, its warps over the slabs).
-template <typename T, int kVec>
+// channel gradients.
+template <typename T, int kVec, bool kOne, int kAct>
 __global__ void __launch_bounds__(kThreads) grad_apply_kernel(const Params p) {
+    constexpr int kStat = kOne ? 1 : kVec;
     extern __shared__ float s_group[];  // means of w dz, then of w dz xhat
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t parts = static_cast<int64_t>(p.n) * p.slabs;
     if (blockIdx.x >= parts) {
-        __shared__ float2 s_part[kWarps][32];
-        const int ch = static_cast<int>(blockIdx.x - parts) * 32 + lane;
-        float sum = 0.0f, sumx = 0.0f;
-        if (ch < p.c)
-            for (int64_t i = warp; i < parts; i += kWarps) {
-                const float2 v = p.chan_part[i * p.c + ch];
-                sum += v.x;
-                sumx += v.y;
-            }
-        s_part[warp][lane] = make_float2(sum, sumx);
-        __syncthreads();
-        if (warp == 0 && ch < p.c) {
-            for (int i = 1; i < kWarps; ++i) {
-                sum += s_part[i][lane].x;
-                sumx += s_part[i][lane].y;
-            }
-            if (p.dbias) p.dbias[ch] = sum;
-            if (p.dweight) p.dweight[ch] = sumx;
-        }
+        join_channels(p, parts, static_cast<int>(blockIdx.x - parts) * 32);
         return;
     }
     const Place a = place(p);
@@ -393,41 +450,129 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(const Params p) {
     }
     __syncthreads();
     const int cols = p.c / kVec;
-    const int64_t start = (a.sample * p.rows + a.row0) * p.c;
-    const float* stats = p.stats + static_cast<int64_t>(a.sample) * p.groups * 2;
     for (int col0 = 0; col0 < cols; col0 += kThreads) {
         const int tile = min(cols - col0, kThreads);
         const int lanes = kThreads / tile;
         const int tx = threadIdx.x % tile, ty = threadIdx.x / tile;
         if (ty >= lanes) continue;
         const int c0 = (col0 + tx) * kVec;
-        float mean[kVec], rstd[kVec], w[kVec], bias[kVec], m1[kVec], m2[kVec];
+        Channels<kVec, kOne> ch;
+        ch.load(p, a.sample, c0);
+        float m1[kStat], m2[kStat];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            const int g = (c0 + i) / p.per;
-            mean[i] = stats[2 * g];
-            rstd[i] = stats[2 * g + 1];
-            w[i] = param_at(p.weight, p.param_type, c0 + i, 1.0f);
-            bias[i] = param_at(p.bias, p.param_type, c0 + i, 0.0f);
-            m1[i] = s_group[g];
-            m2[i] = s_group[p.groups + g];
+        for (int i = 0; i < kStat; ++i) {
+            m1[i] = s_group[(c0 + i) / p.per];
+            m2[i] = s_group[p.groups + (c0 + i) / p.per];
         }
-        const T* x = static_cast<const T*>(p.x) + start + c0;
-        const T* dy = static_cast<const T*>(p.dy) + start + c0;
-        T* out = static_cast<T*>(p.out) + start + c0;
+        const int64_t first = a.start + static_cast<int64_t>(ty) * p.c + c0, step = static_cast<int64_t>(lanes) * p.c;
+        const T* x = static_cast<const T*>(p.x) + first;
+        const T* dy = static_cast<const T*>(p.dy) + first;
+        T* out = static_cast<T*>(p.out) + first;
 #pragma unroll 2
-        for (int64_t r = ty; r < a.rows; r += lanes) {
+        for (int r = ty; r < a.rows; r += lanes, x += step, dy += step, out += step) {
             float v[kVec], d[kVec];
-            load_f32<T, kVec>(x + r * p.c, v);
-            load_f32<T, kVec>(dy + r * p.c, d);
+            load_f32<T, kVec>(x, v);
+            load_f32<T, kVec>(dy, d);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                const float xhat = (v[i] - mean[i]) * rstd[i];
-                const float dz = d[i] * slope(fmaf(xhat, w[i], bias[i]), p.act);
-                v[i] = rstd[i] * (fmaf(w[i], dz, -m1[i]) - xhat * m2[i]);
+                const int k = kOne ? 0 : i;
+                const float2 g = ch.template at<kAct>(p, i, v[i], d[i]);
+                v[i] = ch.rstd[k] * (fmaf(ch.w[i], g.y, -m1[k]) - g.x * m2[k]);
             }
-            store_f32<T, kVec>(out + r * p.c, v);
+            store_f32<T, kVec>(out, v);
         }
+    }
+}
+
+// ------------------------------------------------- samples of one block each
+
+// A block a sample whose slab fits shared memory: one copy in, two sums over
+// it (the mean, then the squared distances from it), one result out.
+constexpr int kSmallBytes = 65536;
+
+// Sums v over the threads of each group (whole vectors); every thread of the
+// group gets its sum. s: a float a thread and a group.
+__device__ __forceinline__ float group_sum(float v, float* s, int cols, int lanes, int width, int groups, int group) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    s[threadIdx.x] = v;
+    __syncthreads();
+    const float inv = 1.0f / static_cast<float>(width);
+    for (int g = warp; g < groups; g += kWarps) {
+        float x = 0.0f;
+        for (int e = lane; e < width * lanes; e += 32) {
+            const int row = quotient(e, inv);
+            x += s[row * cols + g * width + e - row * width];
+        }
+        x = warp_sum(x);
+        if (lane == 0) s[kThreads + g] = x;
+    }
+    __syncthreads();
+    return group < groups ? s[kThreads + group] : 0.0f;
+}
+
+template <typename T, int kVec, int kAct>
+__global__ void __launch_bounds__(kThreads) small_kernel(const Params p, uint32_t* status) {
+    extern __shared__ __align__(16) uint8_t smem[];  // the sample
+    __shared__ float s_sum[kThreads + kThreads];
+    __shared__ __align__(8) uint64_t s_full;
+    const int cols = p.c / kVec, lanes = kThreads / cols, width = p.per / kVec, rows = static_cast<int>(p.rows);
+    const int tx = threadIdx.x % cols, ty = threadIdx.x / cols;
+    const int group = ty < lanes ? tx / width : p.groups, c0 = tx * kVec;
+    const int64_t start = static_cast<int64_t>(blockIdx.x) * rows * p.c;
+    if (threadIdx.x == 0) {
+        const uint32_t bytes = static_cast<uint32_t>(rows) * p.c * sizeof(T), bar = smem_addr(&s_full);
+        mbar_init(bar, 1);
+        fence_mbarrier_init();
+        mbar_arrive_expect_tx(bar, bytes);
+        bulk_g2s(smem_addr(smem), static_cast<const T*>(p.x) + start, bytes, bar);
+    }
+    float gain[kVec], bias[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+        gain[i] = ty < lanes ? param_at(p.weight, p.param_type, c0 + i, 1.0f) : 0.0f;
+        bias[i] = ty < lanes ? param_at(p.bias, p.param_type, c0 + i, 0.0f) : 0.0f;
+    }
+    __syncthreads();
+    uint32_t none = 0;
+    if (!mbar_wait(smem_addr(&s_full), 0, &none, status, kStatusTimeoutXFull)) return;
+    const T* x = reinterpret_cast<const T*>(smem) + c0;
+    const int end = ty < lanes ? rows : 0;
+    // distances from the group's first element keep a far mean's digits
+    const float shift = ty < lanes ? to_f32<T>(reinterpret_cast<const T*>(smem)[group * p.per]) : 0.0f;
+    const float inv = 1.0f / (static_cast<float>(rows) * static_cast<float>(p.per));
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int r = ty; r < end; r += lanes) {
+        float v[kVec];
+        load_f32<T, kVec>(x + r * p.c, v);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sum += v[i] - shift;
+    }
+    const float mean = shift + group_sum(sum, s_sum, cols, lanes, width, p.groups, group) * inv;
+    sum = 0.0f;
+#pragma unroll 4
+    for (int r = ty; r < end; r += lanes) {
+        float v[kVec];
+        load_f32<T, kVec>(x + r * p.c, v);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) sum = fmaf(v[i] - mean, v[i] - mean, sum);
+    }
+    const float rstd = 1.0f / sqrtf(group_sum(sum, s_sum, cols, lanes, width, p.groups, group) * inv + p.eps);
+    if (p.stats && ty == 0 && tx % width == 0) {
+        float* out = p.stats + (static_cast<int64_t>(blockIdx.x) * p.groups + group) * 2;
+        out[0] = mean;
+        out[1] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) gain[i] *= rstd;
+    T* y = static_cast<T*>(p.out) + start + c0;
+#pragma unroll 2
+    for (int r = ty; r < end; r += lanes) {
+        float v[kVec];
+        load_f32<T, kVec>(x + r * p.c, v);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(v[i] - mean, gain[i], bias[i]), act_of<kAct>(p));
+        store_f32<T, kVec>(y + static_cast<int64_t>(r) * p.c, v);
     }
 }
 
