@@ -66,26 +66,68 @@ __device__ __forceinline__ float param_at(const void* p, int type, int i, float 
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-// Two exponential-unit instructions; both are within 2 units in the last
-// place, so the result is within about 4.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == kRelu) return z < 0.0f ? 0.0f : z;  // keeps a NaN
-    if (act == kSilu) return z * sigmoid(z);
-    if (act == kGelu) return z * (0.5f * (1.0f + erff(z * 0.70710678118654752f)));
-    return z;
+// Two exponential-unit instructions, each within 2 units in the last place
+// (and the product's rounding in the exponent), as the bound of the forward
+// and backward passes is close to that unit: 1 / (1 + 2^(-z log2 e)).
+__device__ __forceinline__ void sigmoid2(float& x, float& y) {
+    constexpr float kNegLog2e = -1.4426950408889634f;
+    mul2(x, y, kNegLog2e, kNegLog2e);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+    add2(x, y, 1.0f, 1.0f);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(y));
 }
 
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == kRelu) return z > 0.0f ? 1.0f : 0.0f;
-    if (act == kSilu) {
-        const float s = sigmoid(z);
-        return s * (1.0f + z * (1.0f - s));
+// z to act(z), two at a time.
+__device__ __forceinline__ void activate2(float& x, float& y, int act) {
+    if (act == kRelu) {
+        x = x < 0.0f ? 0.0f : x;  // keeps a NaN
+        y = y < 0.0f ? 0.0f : y;
+    } else if (act == kSilu) {
+        float s0 = x, s1 = y;
+        sigmoid2(s0, s1);
+        mul2(x, y, s0, s1);
+    } else if (act == kGelu) {
+        x *= 0.5f * (1.0f + erff(x * 0.70710678118654752f));
+        y *= 0.5f * (1.0f + erff(y * 0.70710678118654752f));
     }
-    if (act == kGelu)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
-    return 1.0f;
+}
+
+// z to act'(z), two at a time.
+__device__ __forceinline__ void slope2(float& x, float& y, int act) {
+    if (act == kRelu) {
+        x = x > 0.0f ? 1.0f : 0.0f;
+        y = y > 0.0f ? 1.0f : 0.0f;
+    } else if (act == kSilu) {  // s (1 + z (1 - s))
+        float s0 = x, s1 = y;
+        sigmoid2(s0, s1);
+        float t0 = s0, t1 = s1;
+        fma2(t0, t1, -1.0f, -1.0f, 1.0f, 1.0f);
+        fma2(x, y, t0, t1, 1.0f, 1.0f);
+        mul2(x, y, s0, s1);
+    } else if (act == kGelu) {
+        auto one = [](float z) {
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+        };
+        x = one(x);
+        y = one(y);
+    } else {
+        x = y = 1.0f;
+    }
+}
+
+// f(v0, v1, i, j) over a vector's elements in pairs; a single element has
+// itself as its partner's index and a partner that nothing reads.
+template <int kVec, typename F>
+__device__ __forceinline__ void in_pairs(float (&v)[kVec], F&& f) {
+    if constexpr (kVec == 1) {
+        float none = 0.0f;
+        f(v[0], none, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2) f(v[i], v[i + 1], i, i + 1);
+    }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -279,9 +321,11 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(const Params p) {
         for (int r = ty; r < a.rows; r += lanes, in += step, out += step) {
             float v[kVec];
             load_f32<T, kVec>(in, v);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i)
-                v[i] = activate(fmaf(v[i] - mean[kOne ? 0 : i], gain[i], bias[i]), act_of<kAct>(p));
+            in_pairs<kVec>(v, [&](float& x, float& y, int i, int j) {
+                add2(x, y, -mean[kOne ? 0 : i], -mean[kOne ? 0 : j]);
+                fma2(x, y, gain[i], gain[j], bias[i], bias[j]);
+                activate2(x, y, act_of<kAct>(p));
+            });
             store_f32<T, kVec>(out, v);
         }
     }
@@ -306,12 +350,16 @@ struct Channels {
             bias[i] = param_at(p.bias, p.param_type, c0 + i, 0.0f);
         }
     }
-    // xhat and dz of channel i
+    // x to xhat and dy to dz of channels i and j
     template <int kAct>
-    __device__ __forceinline__ float2 at(const Params& p, int i, float x, float dy) const {
-        const int k = kOne ? 0 : i;
-        const float xhat = (x - mean[k]) * rstd[k];
-        return make_float2(xhat, dy * slope(fmaf(xhat, w[i], bias[i]), act_of<kAct>(p)));
+    __device__ __forceinline__ void at(const Params& p, int i, int j, float& x0, float& x1, float& d0, float& d1) const {
+        const int k = kOne ? 0 : i, l = kOne ? 0 : j;
+        add2(x0, x1, -mean[k], -mean[l]);
+        mul2(x0, x1, rstd[k], rstd[l]);
+        float z0 = x0, z1 = x1;
+        fma2(z0, z1, w[i], w[j], bias[i], bias[j]);
+        slope2(z0, z1, act_of<kAct>(p));
+        mul2(d0, d1, z0, z1);
     }
 };
 
@@ -341,12 +389,18 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const Params p) {
                 float v[kVec], d[kVec];
                 load_f32<T, kVec>(x, v);
                 load_f32<T, kVec>(dy, d);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float2 g = ch.template at<kAct>(p, i, v[i], d[i]);
-                    sdz[i] += g.y;
-                    sdzx[i] = fmaf(g.y, g.x, sdzx[i]);
-                }
+                in_pairs<kVec>(v, [&](float& x0, float& x1, int i, int j) {
+                    float d0 = d[i], d1 = d[j];
+                    ch.template at<kAct>(p, i, j, x0, x1, d0, d1);
+                    if constexpr (kVec == 1) {
+                        sdz[0] += d0;
+                        sdzx[0] = fmaf(d0, x0, sdzx[0]);
+                    } else {
+                        fma2(x0, x1, d0, d1, sdzx[i], sdzx[j]);
+                        sdzx[i] = x0, sdzx[j] = x1;
+                        add2(sdz[i], sdz[j], d0, d1);
+                    }
+                });
             }
         }
 #pragma unroll
@@ -473,12 +527,14 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(const Params p) {
             float v[kVec], d[kVec];
             load_f32<T, kVec>(x, v);
             load_f32<T, kVec>(dy, d);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                const int k = kOne ? 0 : i;
-                const float2 g = ch.template at<kAct>(p, i, v[i], d[i]);
-                v[i] = ch.rstd[k] * (fmaf(ch.w[i], g.y, -m1[k]) - g.x * m2[k]);
-            }
+            in_pairs<kVec>(v, [&](float& x0, float& x1, int i, int j) {
+                const int k = kOne ? 0 : i, l = kOne ? 0 : j;
+                float d0 = d[i], d1 = d[j];
+                ch.template at<kAct>(p, i, j, x0, x1, d0, d1);
+                fma2(d0, d1, ch.w[i], ch.w[j], -m1[k], -m1[l]);
+                fma2(x0, x1, -m2[k], -m2[l], d0, d1);
+                mul2(x0, x1, ch.rstd[k], ch.rstd[l]);
+            });
             store_f32<T, kVec>(out, v);
         }
     }
@@ -570,8 +626,11 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const Params p, uint32_
     for (int r = ty; r < end; r += lanes) {
         float v[kVec];
         load_f32<T, kVec>(x + r * p.c, v);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(v[i] - mean, gain[i], bias[i]), act_of<kAct>(p));
+        in_pairs<kVec>(v, [&](float& x, float& y, int i, int j) {
+            add2(x, y, -mean, -mean);
+            fma2(x, y, gain[i], gain[j], bias[i], bias[j]);
+            activate2(x, y, act_of<kAct>(p));
+        });
         store_f32<T, kVec>(y + static_cast<int64_t>(r) * p.c, v);
     }
 }

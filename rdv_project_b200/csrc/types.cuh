@@ -38,6 +38,29 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 
+// Two float32 operations in one packed instruction (sm_100): (a0, a1) op
+// (b0, b1) into the first pair, and a b + c.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a0, a1)), "l"(pair_of(b0, b1)));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(d));
+}
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a0, a1)), "l"(pair_of(b0, b1)));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(d));
+}
+__device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_of(a0, a1)), "l"(pair_of(b0, b1)), "l"(pair_of(c0, c1)));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(d));
+}
+
 // N consecutive elements moved as one access (N * sizeof(T) is 1 to 16 bytes
 // and the address a multiple of it).
 template <typename T, int N>
