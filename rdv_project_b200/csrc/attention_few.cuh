@@ -23,7 +23,7 @@ constexpr int kFewThreads = 128, kFewWarps = kFewThreads / 32, kFewRows = 8;
 
 // (c0, c1) += (a0 b0, a1 b1) in one packed instruction.
 __device__ __forceinline__ void fma_f32x2_acc(float& c0, float& c1, float a0, float a1, float b0, float b1) {
-    fma_f32x2(a0, a1, b0, b1, c0, c1);
+    fma2(a0, a1, b0, b1, c0, c1);
     c0 = a0;
     c1 = a1;
 }

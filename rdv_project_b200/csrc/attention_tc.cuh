@@ -167,69 +167,57 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// (a0, a1) * (b0, b1) in one packed instruction.
-__device__ __forceinline__ void mul_f32x2(float& a0, float& a1, float b0, float b1) {
-    uint64_t pa, pb, pd;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b0), "f"(b1));
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(pd) : "l"(pa), "l"(pb));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
-}
-// (a0 b0 + c0, a1 b1 + c1) in one packed instruction.
-__device__ __forceinline__ void fma_f32x2(float& a0, float& a1, float b0, float b1, float c0, float c1) {
-    uint64_t pa, pb, pc, pd;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b0), "f"(b1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pc) : "f"(c0), "f"(c1));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(pd) : "l"(pa), "l"(pb), "l"(pc));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
-}
-// (a0 b + c, a1 b + c) in one packed instruction.
-__device__ __forceinline__ void fma_f32x2(float& a0, float& a1, float b, float c) {
-    uint64_t pa, pb, pc, pd;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a0), "f"(a1));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(pb) : "f"(b));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(pc) : "f"(c));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(pd) : "l"(pa), "l"(pb), "l"(pc));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(pd));
-}
-
 // Which of the 128 keys from k0 on are allowed, as four words; the same in
-// every lane of a warp. Call with all 32 lanes.
+// every lane of a warp. key_load reads the mask's bytes (a lane's four), so
+// that a loop can have them on their way for its next step; key_bits votes.
+// Call both with all 32 lanes.
 struct KeyBits {
     uint32_t w[4];
     __device__ __forceinline__ bool all() const { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
     __device__ __forceinline__ bool none() const { return (w[0] | w[1] | w[2] | w[3]) == 0u; }
 };
-__device__ __forceinline__ KeyBits key_bits(const Params& p, int b, int64_t k0, int64_t end) {
-    KeyBits bits;
+struct KeyLoad {
+    int left;  // keys from k0 to the end, at most 128
+    uint8_t m[4];
+};
+__device__ __forceinline__ KeyLoad key_load(const Params& p, int b, int64_t k0, int64_t end) {
+    KeyLoad l;
     const int64_t left = end - k0;
+    l.left = left < 0 ? 0 : left < 128 ? static_cast<int>(left) : 128;
     const int lane = threadIdx.x & 31;
 #pragma unroll
+    for (int i = 0; i < 4; ++i)
+        l.m[i] = p.mask && 32 * i + lane < l.left ? p.mask[b * p.mask_stride + k0 + 32 * i + lane] : 0;
+    return l;
+}
+__device__ __forceinline__ KeyBits key_bits(const Params& p, const KeyLoad& l) {
+    KeyBits bits;
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t n = left - 32 * i;
-        uint32_t w = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
-        if (p.mask) {
-            const bool in = 32 * i + lane < left;
-            w = __ballot_sync(0xffffffffu, in && p.mask[b * p.mask_stride + k0 + 32 * i + lane] != 0);
-        }
-        bits.w[i] = w;
+        const int n = l.left - 32 * i;
+        if (p.mask)
+            bits.w[i] = __ballot_sync(0xffffffffu, l.m[i] != 0);
+        else
+            bits.w[i] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
     }
     return bits;
 }
 
 // Zeroes the rows of a 128-row tile (atoms of 64 elements, kAtoms of them)
-// whose bit is not set. Call with all 32 lanes of one warp, then fence.
+// whose bit is not set: a lane a row, 16 bytes a store, its columns turned so
+// that the lanes' banks differ. Call with all 32 lanes of one warp, then fence.
 template <int kAtoms>
 __device__ __forceinline__ void zero_rows(uint32_t tile, const KeyBits& bits) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        for (uint32_t off = ~bits.w[i]; off; off &= off - 1) {
-            const uint32_t row = 32 * i + __ffs(off) - 1;
-            if (lane < 8 * kAtoms)
-                st_shared_v4(tile + (lane >> 3) * (kTcTile * 128) + row * 128 + (lane & 7) * 16, 0, 0, 0, 0);
-        }
+    for (int i = 0; i < 4; ++i) {
+        if (bits.w[i] == 0xffffffffu) continue;
+        if (bits.w[i] >> lane & 1u) continue;
+        const uint32_t row = tile + (32 * i + lane) * 128;
+#pragma unroll
+        for (int j = 0; j < 8 * kAtoms; ++j)
+            st_shared_v4(row + (j >> 3) * (kTcTile * 128) + ((j + lane) & 7) * 16, 0, 0, 0, 0);
+    }
 }
 
 // A block's place in the forward pass and dQ: query tile, head, sample,
@@ -265,19 +253,29 @@ __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
     asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x));  // -127
     asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y));
     float n0 = x, n1 = y;
-    add_f32x2(n0, n1, kRound, kRound);
+    add2(n0, n1, kRound, kRound);
     const float s0 = __uint_as_float(__float_as_uint(n0) << 23), s1 = __uint_as_float(__float_as_uint(n1) << 23);
-    add_f32x2(n0, n1, -kRound, -kRound);
+    add2(n0, n1, -kRound, -kRound);
     float f0 = n0, f1 = n1;
-    fma_f32x2(f0, f1, -1.0f, -1.0f, x, y);
+    fma2(f0, f1, -1.0f, -1.0f, x, y);
     float p0 = f0, p1 = f1;
-    fma_f32x2(p0, p1, 0.009570101908f, 0.05591786032f);
-    fma_f32x2(p0, p1, f0, f1, 0.2402474483f, 0.2402474483f);
-    fma_f32x2(p0, p1, f0, f1, 0.6931218147f, 0.6931218147f);
-    fma_f32x2(p0, p1, f0, f1, 0.9999992614f, 0.9999992614f);
-    mul_f32x2(p0, p1, s0, s1);
+    fma2(p0, p1, 0.009570101908f, 0.009570101908f, 0.05591786032f, 0.05591786032f);
+    fma2(p0, p1, f0, f1, 0.2402474483f, 0.2402474483f);
+    fma2(p0, p1, f0, f1, 0.6931218147f, 0.6931218147f);
+    fma2(p0, p1, f0, f1, 0.9999992614f, 0.9999992614f);
+    mul2(p0, p1, s0, s1);
     x = p0;
     y = p1;
+}
+// 2^x and 2^y: `poly` of every four pairs by the polynomial.
+template <int kPoly>
+__device__ __forceinline__ void exp2_pair(float& x, float& y, int pair) {
+    if (pair % 4 >= 4 - kPoly) {
+        exp2_poly2(x, y);
+    } else {
+        x = exp2_approx(x);
+        y = exp2_approx(y);
+    }
 }
 
 template <int DP>
@@ -292,9 +290,9 @@ struct TcForward {
     static constexpr uint32_t kOffK = 2 * kTileBytes, kOffV = kOffK + kStages * kTileBytes,
                               kOffBar = kOffV + kStages * kTileBytes;
     static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // barriers; slack for the 1024-byte alignment
-    // Of eight pairs of exponentials, those taken by the polynomial: at 64
+    // Of four pairs of exponentials, those taken by the polynomial: at 64
     // dimensions the exponential unit is what the products wait for.
-    static constexpr int kPolyPairs = DP == 64 ? 2 : 0;
+    static constexpr int kPoly = DP == 64 ? 1 : 0;
 };
 
 // An item of the forward pass: 256 query rows of one head over the keys of
@@ -502,10 +500,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t n = 0, id = blockIdx.x;
                 TcItem t;
                 bool ok = true;
-                for (; ok && next_item(a, items, id, t); id += gridDim.x)
+                for (; ok && next_item(a, items, id, t); id += gridDim.x) {
+                    KeyLoad keys = key_load(a, t.b, t.begin, t.end);
                     for (int i = 0; i < t.tiles; ++i, ++n) {
                         const uint32_t s = n % kStages;
-                        const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+                        const KeyBits bits = key_bits(a, keys);
+                        keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
                         ok = mbar_wait_warp(v_tma + 8 * s, (n / kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull);
                         if (!ok) break;
                         if (!bits.all()) {
@@ -515,6 +515,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         if (lane == 0) mbar_arrive(v_full + 8 * s);
                     }
+                }
             }
         }
     } else {
@@ -531,8 +532,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (w && !t.both) continue;
             float top = -INFINITY, total = 0.0f;
             bool any = false;
+            KeyLoad keys = key_load(a, t.b, t.begin, t.end);
             for (int i = 0; i < t.tiles; ++i, ++n) {
-                const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+                const KeyBits bits = key_bits(a, keys);
+                keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
                 const bool whole = bits.all();
                 any |= !bits.none();
                 if (!(ok = mbar_wait_warp(s_full + 8 * w, n & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
@@ -595,14 +598,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
-                        fma_f32x2(x, y, c, minus);
-                        if (e / 2 % 4 == 3 && F::kPolyPairs > e / 8) {
-                            exp2_poly2(x, y);
-                        } else {
-                            x = exp2_approx(x);
-                            y = exp2_approx(y);
-                        }
-                        add_f32x2(sum[e & 2], sum[(e & 2) + 1], x, y);
+                        fma2(x, y, c, c, minus, minus);
+                        exp2_pair<F::kPoly>(x, y, e / 2);
+                        add2(sum[e & 2], sum[(e & 2) + 1], x, y);
                         packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
                     }
                     tmem_st8(col_p + 8 * j, packed);

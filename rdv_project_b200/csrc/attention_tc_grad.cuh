@@ -6,8 +6,11 @@
 // instead of the five of one kernel that adds dQ up in memory, and no
 // atomics. One block a processor, 512 TMEM columns. Warps 0-7: probabilities
 // and score gradients, a thread a row (a lane of TMEM) and half the columns.
-// Warp 8: loads. Warp 9: products. Warp 10: zeroes rows of K whose keys are
-// not allowed (dQ).
+// Warp 8: loads. Warp 9: the products S and dP. Warp 11: the products that
+// take P and dS. Warp 10: zeroes rows of K whose keys are not allowed (dQ). A
+// barrier that its producer could complete twice before a slow reader looked
+// (the readers tell phases apart by parity) comes in two, for even and odd
+// tiles.
 //
 // P and dS are rounded to the inputs' type, as the tensor cores take them.
 // float16 has few exponents: P is held times 2^15 (P <= 1), dS times 2^E with
@@ -23,6 +26,7 @@ namespace attn {
 
 constexpr int kGradThreads = 12 * 32;
 constexpr int kPrepBlocks = 296;
+constexpr int kGradPoly = 1;  // of four pairs of exponentials, those taken by the polynomial
 
 struct GradParams {
     Params a;
@@ -180,9 +184,9 @@ __device__ __forceinline__ void store_columns(const Params& a, void* out, float*
 
 // ------------------------------------------------------------------------ dQ
 //
-// A block: 128 query rows of one head over the keys of one split. The
-// products run in the order dQ(i), dP(i + 1), S(i + 2): S has two buffers
-// (dS(i) replaces S(i)), dP one.
+// A block: 128 query rows of one head over the keys of one split. S has two
+// buffers (dS(i) replaces S(i)), dP one: S(i + 1) and dP(i + 1) run beside the
+// exponentials of i and dQ(i).
 template <int DP>
 struct TcDq {
     static constexpr int kAtoms = DP / 64, kKStages = 3, kVStages = 2;
@@ -202,12 +206,12 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t s_q = base, s_do = base + F::kOffDo, s_k = base + F::kOffK, s_v = base + F::kOffV,
                    bars = base + F::kOffBar;
-    const uint32_t q_full = bars, dp_full = bars + 8, ds_full = bars + 16, dq_done = bars + 24, drain = bars + 32,
-                   s_full = bars + 40, k_tma = bars + 56, k_ok = bars + 80, k_empty = bars + 104,
-                   v_full = bars + 128, v_empty = bars + 144;
-    const uint32_t tmem_slot = bars + 160;
+    const uint32_t q_full = bars, dp_full = bars + 8, drain = bars + 16, s_full = bars + 24, ds_full = bars + 40,
+                   dq_done = bars + 56, k_tma = bars + 72, k_ok = bars + 96, k_empty = bars + 120,
+                   v_full = bars + 144, v_empty = bars + 160;
+    const uint32_t tmem_slot = bars + 176;
     volatile uint32_t* abort_flag =
-        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 164);
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 180);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Params& a = p.a;
     const TcPlace t = tc_place(a);
@@ -216,11 +220,11 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         *abort_flag = 0u;
         mbar_init(q_full, 2);  // Q and dO
         mbar_init(dp_full, 1);
-        mbar_init(ds_full, 8);
-        mbar_init(dq_done, 1);
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);  // an arrival an issuing warp
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
+            mbar_init(ds_full + 8 * i, 8);
+            mbar_init(dq_done + 8 * i, 1);
             mbar_init(v_full + 8 * i, 1);
             mbar_init(v_empty + 8 * i, 1);
         }
@@ -264,52 +268,66 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     } else if (warp == 9) {
         if (lane == 0 && t.tiles > 0) {
             const uint32_t idesc = umma_idesc_f16(kTcTile, kBf16);
-            const uint32_t idesc_q = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
             const uint32_t k_ready = p.guarded ? k_ok : k_tma;
-            auto score = [&](int i) {
-                const int s = i % F::kKStages;
+            const uint32_t q_desc = desc_k_major(s_q), do_desc = desc_k_major(s_do), k_desc = desc_k_major(s_k),
+                           v_desc = desc_k_major(s_v);
+            auto score = [&](int i) {  // S(i), over dS(i - 2)
+                const uint32_t s = i % F::kKStages, half = i & 1;
+                if (i >= 2 &&
+                    !mbar_wait(dq_done + 8 * half, (i / 2 - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull))
+                    return false;
                 if (!mbar_wait(k_ready + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows<DP / 16>(tmem + F::kColS + (i & 1) * 128, desc_k_major(s_q),
-                                      desc_k_major(s_k + s * F::kTileBytes), p.k_steps, idesc);
-                umma_commit(s_full + 8 * (i & 1));
+                product_rows<DP / 16>(tmem + F::kColS + half * 128, q_desc, k_desc + s * (F::kTileBytes / 16), p.k_steps,
+                                      idesc);
+                umma_commit(s_full + 8 * half);
                 return true;
             };
-            auto reach = [&](int i) {  // dP(i)
-                const int s = i % F::kVStages;
+            auto reach = [&](int i) {  // dP(i), over dP(i - 1), which was read before dS(i - 1) was complete
+                const uint32_t s = i % F::kVStages;
+                if (i >= 1 && !mbar_wait(ds_full + 8 * ((i - 1) & 1), ((i - 1) / 2) & 1, abort_flag, p.status,
+                                         kStatusTimeoutAFull))
+                    return false;
                 if (!mbar_wait(v_full + 8 * s, (i / F::kVStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows<DP / 16>(tmem + F::kColDp, desc_k_major(s_do), desc_k_major(s_v + s * F::kTileBytes),
-                                      p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::kColDp, do_desc, v_desc + s * (F::kTileBytes / 16), p.k_steps, idesc);
                 umma_commit(v_empty + 8 * s);
                 umma_commit(dp_full);
                 return true;
             };
-            bool ok = mbar_wait(q_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0) && reach(0);
-            if (t.tiles > 1) ok = ok && score(1);
+            bool ok = mbar_wait(q_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0);
             for (int i = 0; ok && i < t.tiles; ++i) {
-                const int s = i % F::kKStages;
-                ok = mbar_wait(ds_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull);
-                if (!ok) break;
+                ok = reach(i);
+                if (ok && i + 1 < t.tiles) ok = score(i + 1);
+            }
+            umma_commit(drain);
+            drain_wait(drain, 0, p.status);
+        }
+    } else if (warp == 11) {
+        if (lane == 0 && t.tiles > 0) {
+            const uint32_t idesc = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
+            const uint32_t k_desc = desc_mn_major(s_k);
+            for (int i = 0; i < t.tiles; ++i) {
+                const uint32_t s = i % F::kKStages, half = i & 1;
+                if (!mbar_wait(ds_full + 8 * half, (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull)) break;
                 tc_fence_after();
-                product_columns(tmem + F::kColDq, tmem + F::kColS + (i & 1) * 128,
-                                desc_mn_major(s_k + s * F::kTileBytes), idesc_q, i == 0);
+                product_columns(tmem + F::kColDq, tmem + F::kColS + half * 128, k_desc + s * (F::kTileBytes / 16), idesc,
+                                i == 0);
                 umma_commit(k_empty + 8 * s);
-                umma_commit(dq_done);
-                if (i + 1 < t.tiles) ok = reach(i + 1);  // dP(i) was read before ds_full
-                if (ok && i + 2 < t.tiles)
-                    ok = mbar_wait(dq_done, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && score(i + 2);
+                umma_commit(dq_done + 8 * half);
             }
             umma_commit(drain);
             drain_wait(drain, 0, p.status);
         }
     } else if (warp == 10) {
         if (p.guarded) {
+            KeyLoad keys = key_load(a, t.b, t.begin, t.end);
             for (int i = 0; i < t.tiles; ++i) {
                 const int s = i % F::kKStages;
-                const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+                const KeyBits bits = key_bits(a, keys);
+                keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
                 if (!mbar_wait_warp(k_tma + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     break;
                 if (!bits.all()) {
@@ -329,8 +347,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const int64_t stat = (static_cast<int64_t>(t.b) * a.heads + t.h) * p.q_pad + q;
         const float minus = p.neg_lse[stat] + e2, neg_delta = p.neg_delta[stat];
         bool ok = true, any = false;
+        KeyLoad keys = key_load(a, t.b, t.begin, t.end);
         for (int i = 0; i < t.tiles; ++i) {
-            const KeyBits bits = key_bits(a, t.b, t.begin + static_cast<int64_t>(i) * kTcTile, t.end);
+            const KeyBits bits = key_bits(a, keys);
+            keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
             const bool whole = bits.all();
             any |= !bits.none();
             const uint32_t s_col = row_base + F::kColS + (i & 1) * 128 + half * 64;
@@ -347,9 +367,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
-                    fma_f32x2(x, y, c, minus);
-                    r[j][e] = __float_as_uint(exp2_approx(x));
-                    r[j][e + 1] = __float_as_uint(exp2_approx(y));
+                    fma2(x, y, c, c, minus, minus);
+                    exp2_pair<kGradPoly>(x, y, e / 2);
+                    r[j][e] = __float_as_uint(x);
+                    r[j][e + 1] = __float_as_uint(y);
                 }
             if (!(ok = mbar_wait_warp(dp_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
             tc_fence_after();
@@ -362,8 +383,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float x = __uint_as_float(d[e]), y = __uint_as_float(d[e + 1]);
-                    add_f32x2(x, y, neg_delta, neg_delta);
-                    mul_f32x2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
+                    add2(x, y, neg_delta, neg_delta);
+                    mul2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
                     if (!whole) {
                         x = word >> e & 1u ? x : 0.0f;
                         y = word >> (e + 1) & 1u ? y : 0.0f;
@@ -375,7 +396,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full);
+            if (lane == 0) mbar_arrive(ds_full + 8 * (i & 1));
         }
         if (t.tiles > 0 && ok) ok = mbar_wait_warp(drain, 0, abort_flag, p.status, kStatusTimeoutAccFull);
         tc_fence_after();
@@ -406,19 +427,23 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 // ------------------------------------------------------------------- dK, dV
 //
 // A block: 128 keys of one key head over the (query head, query tile) pairs
-// of one split, with keys as TMEM lanes: S^T = K Q^T, dP^T = V dO^T, P^T and
-// dS^T replace them, dV += P^T dO, dK += dS^T Q. The products run in the
-// order dV(i), dK(i), S(i + 1), dP(i + 1); the exponentials of i + 1 run while
-// dP(i + 1) does, dS(i) while dV(i) does.
+// of one split, with keys as TMEM lanes: S^T = K Q^T, dP^T = V dO^T, dV += P^T
+// dO, dK += dS^T Q. P(i) and dS(i) go where S(i) was (a half row each). Up to
+// 64 dimensions S has two buffers and dP one, so S(i + 1) is ready when dS(i)
+// is; at 128, where O's columns leave two in all, S(i + 1) takes dP(i)'s as
+// soon as that has been read, and dP(i + 1) S(i)'s once dK(i) has.
 template <int DP>
 struct TcDkv {
-    static constexpr int kAtoms = DP / 64, kStages = 2;
+    static constexpr int kAtoms = DP / 64, kStages = DP == 64 ? 3 : 2;
+    static constexpr bool kSwap = DP == 128;
     static constexpr uint32_t kTileBytes = kTcTile * DP * 2;
     static constexpr uint32_t kOffV = kTileBytes, kOffQ = 2 * kTileBytes, kOffDo = kOffQ + kStages * kTileBytes,
                               kOffStat = kOffDo + kStages * kTileBytes;  // [stage][-lse, -delta][128]
     static constexpr uint32_t kOffBar = kOffStat + kStages * 1024;
-    static constexpr uint32_t kBytes = kOffBar + 256 + 1024;
-    static constexpr uint32_t kColS = 0, kColDp = 128, kColDv = 256, kColDk = 384;
+    static constexpr uint32_t kBytes = kOffBar + 512 + 1024;
+    static constexpr uint32_t kColDv = kSwap ? 256 : 384, kColDk = kSwap ? 384 : 448;
+    static __device__ __forceinline__ uint32_t col_s(int i) { return (i & 1) * 128; }
+    static __device__ __forceinline__ uint32_t col_dp(int i) { return kSwap ? (~i & 1) * 128 : 256; }
 };
 
 template <int DP, bool kBf16>
@@ -430,12 +455,12 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t s_k = base, s_v = base + F::kOffV, s_q = base + F::kOffQ, s_do = base + F::kOffDo,
                    s_stat = base + F::kOffStat, bars = base + F::kOffBar;
-    const uint32_t kv_full = bars, s_full = bars + 8, p_full = bars + 16, dp_full = bars + 24, ds_full = bars + 32,
-                   dv_done = bars + 40, dk_done = bars + 48, drain = bars + 56, q_full = bars + 64,
-                   q_empty = bars + 80, do_full = bars + 96, do_empty = bars + 112;
-    const uint32_t tmem_slot = bars + 128;
+    const uint32_t kv_full = bars, dp_full = bars + 8, dp_read = bars + 16, drain = bars + 24, s_full = bars + 32,
+                   p_full = bars + 48, ds_full = bars + 64, dk_done = bars + 80, q_full = bars + 96,
+                   q_empty = bars + 120, do_full = bars + 144, do_empty = bars + 168;
+    const uint32_t tmem_slot = bars + 192;
     volatile uint32_t* abort_flag =
-        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 132);
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 196);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Params& a = p.a;
     const uint32_t k_tiles = static_cast<uint32_t>((a.kv_len + kTcTile - 1) / kTcTile);
@@ -446,7 +471,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     const int hk = id % a.kv_heads;
     id /= a.kv_heads;
     const int b = id % a.batch, split = id / a.batch;
-    const KeyBits bits = key_bits(a, b, k0, length_of(a, b));
+    const KeyBits bits = key_bits(a, key_load(a, b, k0, length_of(a, b)));
     const int first = static_cast<int>(split * a.split_len);
     const int last = min(q_tiles * a.group, static_cast<int>(first + a.split_len));
     const int items = bits.none() ? 0 : last - first;
@@ -454,13 +479,15 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
         mbar_init(kv_full, 2);
-        mbar_init(s_full, 1);
-        mbar_init(p_full, 8);
         mbar_init(dp_full, 1);
-        mbar_init(ds_full, 8);
-        mbar_init(dv_done, 1);
-        mbar_init(dk_done, 1);
-        mbar_init(drain, 1);
+        mbar_init(dp_read, 8);
+        mbar_init(drain, 2);  // an arrival an issuing warp
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 8);
+            mbar_init(ds_full + 8 * i, 8);
+            mbar_init(dk_done + 8 * i, 1);
+        }
         for (int i = 0; i < F::kStages; ++i) {
             mbar_init(q_full + 8 * i, 2);  // the tile and its -lse
             mbar_init(q_empty + 8 * i, 1);
@@ -507,45 +534,57 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     } else if (warp == 9) {
         if (lane == 0 && items > 0) {
             const uint32_t idesc = umma_idesc_f16(kTcTile, kBf16);
-            const uint32_t idesc_d = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
+            const uint32_t k_desc = desc_k_major(s_k), v_desc = desc_k_major(s_v), q_desc = desc_k_major(s_q),
+                           do_desc = desc_k_major(s_do);
+            // the (i / 2)-th phase of a barrier of even and odd tiles
+            auto wait2 = [&](uint32_t bar, int i, uint32_t code) {
+                return mbar_wait(bar + 8 * (i & 1), (i / 2) & 1, abort_flag, p.status, code);
+            };
             auto score = [&](int i) {
-                const int s = i % F::kStages;
+                const uint32_t s = i % F::kStages;
+                if (F::kSwap ? i >= 1 && !mbar_wait(dp_read, (i - 1) & 1, abort_flag, p.status, kStatusTimeoutAFull)
+                             : i >= 2 && !wait2(dk_done, i - 2, kStatusTimeoutAccFull))
+                    return false;
                 if (!mbar_wait(q_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows<DP / 16>(tmem + F::kColS, desc_k_major(s_k), desc_k_major(s_q + s * F::kTileBytes),
-                                      p.k_steps, idesc);
-                umma_commit(s_full);
+                product_rows<DP / 16>(tmem + F::col_s(i), k_desc, q_desc + s * (F::kTileBytes / 16), p.k_steps, idesc);
+                umma_commit(s_full + 8 * (i & 1));
                 return true;
             };
             auto reach = [&](int i) {
-                const int s = i % F::kStages;
+                const uint32_t s = i % F::kStages;
+                if (i >= 1 && !wait2(F::kSwap ? dk_done : ds_full, i - 1, kStatusTimeoutAccFull)) return false;
                 if (!mbar_wait(do_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows<DP / 16>(tmem + F::kColDp, desc_k_major(s_v), desc_k_major(s_do + s * F::kTileBytes),
-                                      p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::col_dp(i), v_desc, do_desc + s * (F::kTileBytes / 16), p.k_steps, idesc);
                 umma_commit(dp_full);
                 return true;
             };
-            bool ok = mbar_wait(kv_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0) && reach(0);
+            bool ok = mbar_wait(kv_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0);
             for (int i = 0; ok && i < items; ++i) {
-                const int s = i % F::kStages;
-                if (!(ok = mbar_wait(p_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull))) break;
+                ok = reach(i);
+                if (ok && i + 1 < items) ok = score(i + 1);
+            }
+            umma_commit(drain);
+            drain_wait(drain, 0, p.status);
+        }
+    } else if (warp == 11) {
+        if (lane == 0 && items > 0) {
+            const uint32_t idesc = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
+            const uint32_t q_desc = desc_mn_major(s_q), do_desc = desc_mn_major(s_do);
+            for (int i = 0; i < items; ++i) {
+                const uint32_t s = i % F::kStages, half = i & 1, at = s * (F::kTileBytes / 16);
+                if (!mbar_wait(p_full + 8 * half, (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull)) break;
                 tc_fence_after();
-                product_columns(tmem + F::kColDv, tmem + F::kColS, desc_mn_major(s_do + s * F::kTileBytes), idesc_d,
-                                i == 0);
-                umma_commit(do_empty + 8 * s);
-                umma_commit(dv_done);
-                if (!(ok = mbar_wait(ds_full, i & 1, abort_flag, p.status, kStatusTimeoutAFull))) break;
+                product_columns(tmem + F::kColDv, tmem + F::col_s(i), do_desc + at, idesc, i == 0);
+                if (!mbar_wait(ds_full + 8 * half, (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull)) break;
                 tc_fence_after();
-                product_columns(tmem + F::kColDk, tmem + F::kColDp, desc_mn_major(s_q + s * F::kTileBytes), idesc_d,
-                                i == 0);
+                product_columns(tmem + F::kColDk, tmem + F::col_s(i) + 32, q_desc + at, idesc, i == 0);
+                umma_commit(do_empty + 8 * s);  // dS(i) took dP(i), so nothing reads dO(i) any more either
                 umma_commit(q_empty + 8 * s);
-                umma_commit(dk_done);
-                if (i + 1 < items)  // P(i) and dS(i) lie where S(i + 1) and dP(i + 1) go
-                    ok = mbar_wait(dv_done, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && score(i + 1) &&
-                         mbar_wait(dk_done, i & 1, abort_flag, p.status, kStatusTimeoutAccFull) && reach(i + 1);
+                umma_commit(dk_done + 8 * half);
             }
             umma_commit(drain);
             drain_wait(drain, 0, p.status);
@@ -563,15 +602,17 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         bool ok = true;
         for (int i = 0; i < items; ++i) {
             const uint32_t stat = s_stat + (i % F::kStages) * 1024 + half * 256;
-            if (!(ok = mbar_wait_warp(s_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
+            if (!(ok = mbar_wait_warp(s_full + 8 * (i & 1), (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAccFull)))
+                break;
             // the copy of -lse completed with the tile that S(i) was made of; this orders it for this thread
             if (!(ok = mbar_wait_warp(q_full + 8 * (i % F::kStages), (i / F::kStages) & 1, abort_flag, p.status,
                                       kStatusTimeoutXFull)))
                 break;
             tc_fence_after();
+            const uint32_t col = row_base + F::col_s(i) + half * 64;  // P in its first 32 columns, dS in the others
             uint32_t r[2][32];
-            tmem_ld32(row_base + F::kColS + half * 64, r[0]);
-            tmem_ld32(row_base + F::kColS + half * 64 + 32, r[1]);
+            tmem_ld32(col, r[0]);
+            tmem_ld32(col + 32, r[1]);
             tmem_wait_ld32(r[0]);
             reg_barrier32(r[1]);
 #pragma unroll
@@ -583,57 +624,65 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                     if (!kBf16) l.x += kP, l.y += kP, l.z += kP, l.w += kP;
                     float x[4] = {__uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]), __uint_as_float(r[j][e + 2]),
                                   __uint_as_float(r[j][e + 3])};
-                    fma_f32x2(x[0], x[1], c, c, l.x, l.y);
-                    fma_f32x2(x[2], x[3], c, c, l.z, l.w);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] = exp2_approx(x[k]);
+                    fma2(x[0], x[1], c, c, l.x, l.y);
+                    fma2(x[2], x[3], c, c, l.z, l.w);
+                    exp2_pair<kGradPoly>(x[0], x[1], e / 2);
+                    exp2_pair<kGradPoly>(x[2], x[3], e / 2 + 1);
                     packed[e / 2] = kBf16 ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]);
                     packed[e / 2 + 1] = kBf16 ? pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]);
                     if (!kBf16) {
-                        mul_f32x2(x[0], x[1], to_ds, to_ds);
-                        mul_f32x2(x[2], x[3], to_ds, to_ds);
+                        mul2(x[0], x[1], to_ds, to_ds);
+                        mul2(x[2], x[3], to_ds, to_ds);
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) r[j][e + k] = __float_as_uint(x[k]);
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) packed[e] = on ? packed[e] : 0u;
-                tmem_st16(row_base + F::kColS + half * 64 + 16 * j, packed);
+                tmem_st16(col + 16 * j, packed);
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(p_full + 8 * (i & 1));
             if (!(ok = mbar_wait_warp(dp_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
             if (!(ok = mbar_wait_warp(do_full + 8 * (i % F::kStages), (i / F::kStages) & 1, abort_flag, p.status,
                                       kStatusTimeoutXFull)))
                 break;
             tc_fence_after();
+            uint32_t d[2][32];
+            tmem_ld32(row_base + F::col_dp(i) + half * 64, d[0]);
+            tmem_ld32(row_base + F::col_dp(i) + half * 64 + 32, d[1]);
+            tmem_wait_ld32(d[0]);
+            reg_barrier32(d[1]);
+            if (F::kSwap) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(dp_read);
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                uint32_t d[32], packed[16];
-                tmem_ld32(row_base + F::kColDp + half * 64 + 32 * j, d);
-                tmem_wait_ld32(d);
+                uint32_t packed[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
                     const float4 n = ld_shared_f4(stat + 512 + (32 * j + e) * 4);
-                    float x[4] = {__uint_as_float(d[e]), __uint_as_float(d[e + 1]), __uint_as_float(d[e + 2]),
-                                  __uint_as_float(d[e + 3])};
-                    add_f32x2(x[0], x[1], n.x, n.y);
-                    add_f32x2(x[2], x[3], n.z, n.w);
-                    mul_f32x2(x[0], x[1], __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
-                    mul_f32x2(x[2], x[3], __uint_as_float(r[j][e + 2]), __uint_as_float(r[j][e + 3]));
+                    float x[4] = {__uint_as_float(d[j][e]), __uint_as_float(d[j][e + 1]), __uint_as_float(d[j][e + 2]),
+                                  __uint_as_float(d[j][e + 3])};
+                    add2(x[0], x[1], n.x, n.y);
+                    add2(x[2], x[3], n.z, n.w);
+                    mul2(x[0], x[1], __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
+                    mul2(x[2], x[3], __uint_as_float(r[j][e + 2]), __uint_as_float(r[j][e + 3]));
                     packed[e / 2] = kBf16 ? pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]);
                     packed[e / 2 + 1] = kBf16 ? pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]);
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) packed[e] = on ? packed[e] : 0u;
-                tmem_st16(row_base + F::kColDp + half * 64 + 16 * j, packed);
+                tmem_st16(col + 32 + 16 * j, packed);
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full);
+            if (lane == 0) mbar_arrive(ds_full + 8 * (i & 1));
         }
         if (items > 0 && ok) ok = mbar_wait_warp(drain, 0, abort_flag, p.status, kStatusTimeoutAccFull);
         tc_fence_after();
