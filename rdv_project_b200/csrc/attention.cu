@@ -371,7 +371,7 @@ int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void*
         return rc;
     }
     if (p.splits > 1) {
-        const int64_t join = ceil_div(rows, kThreads / 32);
+        const int64_t join = ceil_div(rows * ceil_div(a->dim, 32), kThreads / 32);
         if (int rc = simple_launch_check(join, "join_forward_kernel")) return rc;
         join_forward_kernel<<<static_cast<unsigned>(join), kThreads, 0, st>>>(p);
         return rdvb_host::launched("join_forward_kernel");
@@ -420,9 +420,10 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     p.dk = dk;
     p.dv = dv;
     auto join = [&](const float* part, int splits, int64_t pitch, int64_t n, void* to) -> int {
-        const int64_t blocks = ceil_div(n, kThreads);
+        const int wide = n % 4 == 0 && pitch % 4 == 0 && aligned(part, 16);
+        const int64_t blocks = ceil_div(n, wide ? 4 * kThreads : kThreads);
         if (int rc = simple_launch_check(blocks, "join_kernel")) return rc;
-        join_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(part, splits, pitch, n, to, a->dtype);
+        join_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(part, splits, pitch, n, wide, to, a->dtype);
         return rdvb_host::launched("join_kernel");
     };
     if (l.tc) return launch_tc_backward(a, l, p, workspace, st, join);

@@ -290,13 +290,15 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Params p) {
 
 constexpr int kMaxSplits = 128;
 
-// Joins the splits of the forward pass in split order: a warp a row, a lane
-// up to four splits' weights.
+// Joins the splits of the forward pass in split order: a warp a row's 32
+// dimensions, a lane up to four splits' weights.
 __global__ void __launch_bounds__(kThreads) join_forward_kernel(const Params p) {
     const int64_t rows = static_cast<int64_t>(p.batch) * p.q_len * p.heads;
-    const int64_t row = blockIdx.x * static_cast<int64_t>(kThreads / 32) + threadIdx.x / 32;
+    const int chunks = (p.dim + 31) / 32;
+    const int64_t id = blockIdx.x * static_cast<int64_t>(kThreads / 32) + threadIdx.x / 32;
+    const int64_t row = id / chunks;
     if (row >= rows) return;
-    const int lane = threadIdx.x % 32;
+    const int lane = threadIdx.x % 32, d = static_cast<int>(id % chunks) * 32 + lane;
     constexpr int kMine = kMaxSplits / 32;
     float top = -INFINITY, tops[kMine], totals[kMine];
     bool any = false;
@@ -327,23 +329,19 @@ __global__ void __launch_bounds__(kThreads) join_forward_kernel(const Params p) 
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const float inv = 1.0f / total;
-    for (int d0 = 0; d0 < p.dim; d0 += 32) {
-        const int d = d0 + lane;
-        float acc = 0.0f;
+    float acc = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int n = min(32, p.splits - 32 * i);
-#pragma unroll 4
-            for (int s = 0; s < n; ++s) {
-                const float f = __shfl_sync(0xffffffffu, tops[i], s);
-                // a split without an allowed key has weight 0 and wrote zeros
-                if (d < p.dim) acc = fmaf(p.part[((32 * i + s) * rows + row) * p.dim + d], f, acc);
-            }
+    for (int i = 0; i < kMine; ++i) {
+        const int n = min(32, p.splits - 32 * i);
+#pragma unroll 16
+        for (int s = 0; s < n; ++s) {
+            const float f = __shfl_sync(0xffffffffu, tops[i], s);
+            // a split without an allowed key has weight 0 and wrote zeros
+            if (d < p.dim) acc = fmaf(p.part[((32 * i + s) * rows + row) * p.dim + d], f, acc);
         }
-        if (d < p.dim) store1(p.o, p.dtype, row * p.dim + d, any ? acc * inv : 0.0f);
     }
-    if (lane == 0 && p.lse) {
+    if (d < p.dim) store1(p.o, p.dtype, row * p.dim + d, any ? acc / total : 0.0f);
+    if (d == 0 && p.lse) {
         const int64_t h = row % p.heads, q = row / p.heads % p.q_len, b = row / p.heads / p.q_len;
         p.lse[(b * p.heads + h) * p.q_len + q] = any ? (base + log2f(total)) * kLn2 : -INFINITY;
     }
@@ -543,11 +541,28 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const Params p) {
     }
 }
 
-// Sums `splits` parts of n floats each, `pitch` apart, in split order.
-__global__ void __launch_bounds__(kThreads) join_kernel(const float* part, int splits, int64_t pitch, int64_t n,
+// Sums `splits` parts of n floats each, `pitch` apart, in split order, four
+// elements a thread where `wide` (n and pitch multiples of 4).
+__global__ void __launch_bounds__(kThreads) join_kernel(const float* part, int splits, int64_t pitch, int64_t n, int wide,
                                                         void* out, int dtype) {
-    const int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
+    const int64_t i = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) * (wide ? 4 : 1);
     if (i >= n) return;
+    if (wide) {
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const float4 v = *reinterpret_cast<const float4*>(part + s * pitch + i);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (dtype == 0)
+            store_f32<float, 4>(static_cast<float*>(out) + i, v);
+        else if (dtype == 1)
+            store_f32<__half, 4>(static_cast<__half*>(out) + i, v);
+        else
+            store_f32<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(out) + i, v);
+        return;
+    }
     float sum = 0.0f;
     for (int s = 0; s < splits; ++s) sum += part[s * pitch + i];
     store1(out, dtype, i, sum);

@@ -25,7 +25,7 @@ namespace rdvb {
 namespace attn {
 
 constexpr int kGradThreads = 12 * 32;
-constexpr int kPrepBlocks = 296;
+constexpr int kPrepBlocks = 592;
 constexpr int kGradPoly = 1;  // of four pairs of exponentials, those taken by the polynomial
 
 struct GradParams {
@@ -39,9 +39,11 @@ struct GradParams {
     int guarded;
 };
 
-// neg_lse, neg_delta and norms: kLanes lanes a row, 16 bytes each.
+// neg_lse, neg_delta and norms: kLanes lanes a row of 16 bytes each, in
+// memory order, four rows of dO and O in flight a thread. Bound: memory.
 template <int kLanes, bool kBf16>
 __global__ void __launch_bounds__(kThreads) tc_prep_kernel(const GradParams p) {
+    constexpr int kFlight = 4;
     const Params& a = p.a;
     const int sub = threadIdx.x % kLanes;
     const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / kLanes;
@@ -53,36 +55,62 @@ __global__ void __launch_bounds__(kThreads) tc_prep_kernel(const GradParams p) {
             load_f32<__half, 8>(static_cast<const __half*>(src) + at, v);
     };
     const bool in = sub * 8 < a.dim;
-    const int64_t rows = static_cast<int64_t>(a.batch) * p.q_pad * a.heads;
-    const int64_t rounds = (rows + step - 1) / step;  // the same for every lane of a warp
+    const uint32_t heads = a.heads, length = static_cast<uint32_t>(a.q_len);
+    const int64_t rows = static_cast<int64_t>(a.batch) * length * heads;
+    const int64_t rounds = (rows + step * kFlight - 1) / (step * kFlight);  // the same for every lane of a warp
     float most_do = 0.0f, most_v = 0.0f;
     for (int64_t i = 0; i < rounds; ++i) {
-        const int64_t row = first + i * step;
-        const int64_t h = row % a.heads, q = row / a.heads % p.q_pad, b = row / a.heads / p.q_pad;
-        const bool real = row < rows && q < a.q_len;
-        float dot = 0.0f, norm = 0.0f;
-        if (real && in) {
-            const int64_t at = ((b * a.q_len + q) * a.heads + h) * a.dim + sub * 8;
-            float o[8], g[8];
-            load8(a.out, at, o);
-            load8(a.dout, at, g);
+        uint4 raw_o[kFlight], raw_g[kFlight];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                dot = fmaf(o[j], g[j], dot);
-                norm = fmaf(g[j], g[j], norm);
+        for (int j = 0; j < kFlight; ++j) {
+            const int64_t row = first + (i * kFlight + j) * step;
+            const bool real = row < rows && in;
+            const int64_t at = row * a.dim + sub * 8;
+            raw_o[j] = real ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + at)) : make_uint4(0, 0, 0, 0);
+            raw_g[j] = real ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dout) + at)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kFlight; ++j) {
+            float o[8], g[8], dot = 0.0f, norm = 0.0f;
+            load8(&raw_o[j], 0, o);
+            load8(&raw_g[j], 0, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                dot = fmaf(o[e], g[e], dot);
+                norm = fmaf(g[e], g[e], norm);
             }
-        }
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) {
-            dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            if (!kBf16) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+            for (int e = kLanes / 2; e > 0; e >>= 1) {
+                dot += __shfl_xor_sync(0xffffffffu, dot, e);
+                if (!kBf16) norm += __shfl_xor_sync(0xffffffffu, norm, e);
+            }
+            const int64_t row = first + (i * kFlight + j) * step;
+            if (row < rows && sub == 0) {
+                uint32_t q, h, b;
+                if (rows < 0x100000000LL) {  // 32-bit divisions where they do
+                    const uint32_t r = static_cast<uint32_t>(row);
+                    q = r / heads, h = r - q * heads, b = q / length;
+                    q -= b * length;
+                } else {
+                    h = static_cast<uint32_t>(row % heads);
+                    q = static_cast<uint32_t>(row / heads % length);
+                    b = static_cast<uint32_t>(row / heads / length);
+                }
+                const int64_t head = static_cast<int64_t>(b) * heads + h;
+                p.neg_delta[head * p.q_pad + q] = -dot;
+                p.neg_lse[head * p.q_pad + q] = -a.lse[head * length + q] * kLog2e;
+            }
+            if (!kBf16) most_do = fmaxf(most_do, norm);
         }
-        if (row < rows && sub == 0) {
-            const int64_t at = (b * a.heads + h) * p.q_pad + q;
-            p.neg_delta[at] = real ? -dot : 0.0f;
-            p.neg_lse[at] = real ? -a.lse[(b * a.heads + h) * a.q_len + q] * kLog2e : -INFINITY;
-        }
-        if (!kBf16) most_do = fmaxf(most_do, norm);
+    }
+    // past the end of a head's rows, up to whole tiles
+    const int64_t gap = p.q_pad - a.q_len;
+    const int64_t gaps = gap * a.batch * heads;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < gaps;
+         i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t at = i / gap * p.q_pad + a.q_len + i % gap;
+        p.neg_delta[at] = 0.0f;
+        p.neg_lse[at] = -INFINITY;
     }
     if (kBf16) return;
     const int64_t v_rows = static_cast<int64_t>(a.batch) * a.kv_len * a.kv_heads;

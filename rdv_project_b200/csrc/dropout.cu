@@ -29,7 +29,8 @@ extern "C" int rdvb_dropout(const void* x, const void* residual, void* y, int dt
     a.y = y;
     a.n = n;
     a.offset = offset;
-    a.key = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
+    a.key[0] = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
+    for (int r = 1; r < 10; ++r) a.key[r] = make_uint2(a.key[r - 1].x + 0x9E3779B9u, a.key[r - 1].y + 0xBB67AE85u);
     a.threshold = static_cast<uint32_t>(threshold);
     a.scale = static_cast<float>(1.0 / (1.0 - p));
     const bool wide = aligned(x, 16) && aligned(y, 16) && aligned(residual, 16);
@@ -38,14 +39,17 @@ extern "C" int rdvb_dropout(const void* x, const void* residual, void* y, int dt
     if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "n = %lld is too large", static_cast<long long>(n));
     const unsigned grid = static_cast<unsigned>(blocks);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == RDVB_F32)
-        wide ? dropout_kernel<float, true><<<grid, kThreads, 0, st>>>(a)
-             : dropout_kernel<float, false><<<grid, kThreads, 0, st>>>(a);
-    else if (dtype == RDVB_F16)
-        wide ? dropout_kernel<__half, true><<<grid, kThreads, 0, st>>>(a)
-             : dropout_kernel<__half, false><<<grid, kThreads, 0, st>>>(a);
-    else
-        wide ? dropout_kernel<__nv_bfloat16, true><<<grid, kThreads, 0, st>>>(a)
-             : dropout_kernel<__nv_bfloat16, false><<<grid, kThreads, 0, st>>>(a);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        if (residual)
+            wide ? dropout_kernel<T, true, true><<<grid, kThreads, 0, st>>>(a)
+                 : dropout_kernel<T, false, true><<<grid, kThreads, 0, st>>>(a);
+        else
+            wide ? dropout_kernel<T, true, false><<<grid, kThreads, 0, st>>>(a)
+                 : dropout_kernel<T, false, false><<<grid, kThreads, 0, st>>>(a);
+    };
+    if (dtype == RDVB_F32) go(float{});
+    else if (dtype == RDVB_F16) go(__half{});
+    else go(__nv_bfloat16{});
     return rdvb_host::launched("dropout_kernel");
 }

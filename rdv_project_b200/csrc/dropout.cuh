@@ -4,9 +4,9 @@
 // Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011). The
 // same call on an output gradient is the backward pass.
 //
-// One pass over the data, 16 bytes a thread and access. Bound: memory, and
-// close behind it the 32 x 32 -> 64-bit multiplications (20 a block of four
-// elements).
+// One pass over the data, 16 bytes a thread and access. Bound: the integer
+// pipe -- 19 32 x 32 -> 64-bit multiplications and 20 three-way xors a block of
+// four elements; the rounds' keys come from the host -- a little above memory.
 #pragma once
 #include <cstdint>
 
@@ -17,16 +17,14 @@ namespace dropout {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ uint4 philox(uint64_t counter, uint2 key) {
+__device__ __forceinline__ uint4 philox(uint64_t counter, const uint2 (&key)[10]) {
     uint4 c = make_uint4(static_cast<uint32_t>(counter), static_cast<uint32_t>(counter >> 32), 0u, 0u);
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = static_cast<uint64_t>(c.x) * 0xD2511F53u;
         const uint64_t b = static_cast<uint64_t>(c.z) * 0xCD9E8D57u;
-        c = make_uint4(static_cast<uint32_t>(b >> 32) ^ c.y ^ key.x, static_cast<uint32_t>(b),
-                       static_cast<uint32_t>(a >> 32) ^ c.w ^ key.y, static_cast<uint32_t>(a));
-        key.x += 0x9E3779B9u;
-        key.y += 0xBB67AE85u;
+        c = make_uint4(static_cast<uint32_t>(b >> 32) ^ c.y ^ key[r].x, static_cast<uint32_t>(b),
+                       static_cast<uint32_t>(a >> 32) ^ c.w ^ key[r].y, static_cast<uint32_t>(a));
     }
     return c;
 }
@@ -37,36 +35,36 @@ struct Params {
     void* y;
     int64_t n;
     uint64_t offset;
-    uint2 key;
+    uint2 key[10];       // of each round
     uint32_t threshold;  // kept iff word >= threshold
     float scale;         // 1 / (1 - p)
 };
 
 // kWide: x, residual and y are 16-byte aligned. A thread owns the elements
-// of one 16-byte vector: one block of the generator for float32, two for
-// the 16-bit types. A dropped element is selected to 0, so an infinite or
-// NaN x does not pass the mask. The product and the residual's addition are
-// in float32 and rounded once.
-template <typename T, bool kWide>
+// of one 16-byte vector: one block of the generator for float32, two for the
+// 16-bit types. A dropped element is selected to 0, so an infinite or NaN x
+// does not pass the mask. The product and the residual's addition are in
+// float32 and rounded once.
+template <typename T, bool kWide, bool kResidual>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const Params p) {
     constexpr int kVec = 16 / sizeof(T);
     const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kVec;
     if (i0 >= p.n) return;
-    const T* x = static_cast<const T*>(p.x) + i0;
-    const T* res = p.residual ? static_cast<const T*>(p.residual) + i0 : nullptr;
-    T* y = static_cast<T*>(p.y) + i0;
+    const T* from = static_cast<const T*>(p.x) + i0;
+    const T* add = static_cast<const T*>(p.residual) + i0;
+    T* to = static_cast<T*>(p.y) + i0;
     const bool whole = kWide && i0 + kVec <= p.n;
-    const int count = p.n - i0 < kVec ? static_cast<int>(p.n - i0) : kVec;
-    float v[kVec], r[kVec];
+    Vec<T, kVec> x, res, y;
     if (whole) {
-        load_f32<T, kVec>(x, v);
-        if (res) load_f32<T, kVec>(res, r);
+        x = *reinterpret_cast<const Vec<T, kVec>*>(from);
+        if (kResidual) res = *reinterpret_cast<const Vec<T, kVec>*>(add);
     } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            v[i] = i < count ? to_f32<T>(x[i]) : 0.0f;
-            r[i] = res && i < count ? to_f32<T>(res[i]) : 0.0f;
-        }
+        for (int i = 0; i < kVec; ++i)
+            if (i0 + i < p.n) {
+                x.v[i] = from[i];
+                if (kResidual) res.v[i] = add[i];
+            }
     }
 #pragma unroll
     for (int b = 0; b < kVec / 4; ++b) {
@@ -74,16 +72,16 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const Params p) {
         const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float kept = word[i] >= p.threshold ? v[4 * b + i] * p.scale : 0.0f;
-            v[4 * b + i] = res ? kept + r[4 * b + i] : kept;
+            const float kept = word[i] >= p.threshold ? to_f32<T>(x.v[4 * b + i]) * p.scale : 0.0f;
+            y.v[4 * b + i] = from_f32<T>(kResidual ? kept + to_f32<T>(res.v[4 * b + i]) : kept);
         }
     }
     if (whole) {
-        store_f32<T, kVec>(y, v);
+        *reinterpret_cast<Vec<T, kVec>*>(to) = y;
     } else {
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
-            if (i < count) y[i] = from_f32<T>(v[i]);
+            if (i0 + i < p.n) to[i] = y.v[i];
     }
 }
 
