@@ -121,7 +121,7 @@ struct Plan {
     bool tc, few;
     int forward, dq, dkv;  // splits
     int64_t forward_len, dq_len, dkv_len;
-    int64_t forward_bytes, backward_bytes, delta_bytes, q_pad;
+    int64_t forward_bytes, backward_bytes, delta_bytes, dq_bytes, q_pad;
 };
 
 Plan plan(const rdvb_attention* a) {
@@ -162,7 +162,8 @@ Plan plan(const rdvb_attention* a) {
                          : round16(rows * 4);
     const int64_t dq_bytes = p.dq > 1 ? p.dq * rows * a->dim * 4 : 0;
     const int64_t dkv_bytes = p.dkv > 1 ? 2 * p.dkv * kv_rows * a->dim * 4 : 0;
-    p.backward_bytes = p.delta_bytes + std::max(dq_bytes, dkv_bytes);  // the two are joined in turn
+    p.dq_bytes = round16(dq_bytes);
+    p.backward_bytes = p.delta_bytes + p.dq_bytes + dkv_bytes;
     return p;
 }
 
@@ -195,19 +196,18 @@ void fill(Params& p, const rdvb_attention* a) {
 }
 
 template <typename K>
-int launch(K kernel, int64_t blocks, int smem, const Params& p, cudaStream_t st, const char* what) {
+int launch(K kernel, int64_t blocks, int smem, const Params& p, int device, cudaStream_t st, const char* what) {
     if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute(%s): %s", what, cudaGetErrorString(e));
+    if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), smem, device)) return rc;
     kernel<<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(p);
     return rdvb_host::launched(what);
 }
 
 #define RDVB_BY_DIM(kernel, bytes, ...)                                                                     \
-    (a->dim <= 32    ? launch(kernel<32>, __VA_ARGS__ Shape<32>::bytes, p, st, #kernel)                     \
-     : a->dim <= 64  ? launch(kernel<64>, __VA_ARGS__ Shape<64>::bytes, p, st, #kernel)                     \
-     : a->dim <= 128 ? launch(kernel<128>, __VA_ARGS__ Shape<128>::bytes, p, st, #kernel)                   \
-                     : launch(kernel<256>, __VA_ARGS__ Shape<256>::bytes, p, st, #kernel))
+    (a->dim <= 32    ? launch(kernel<32>, __VA_ARGS__ Shape<32>::bytes, p, dev.index, st, #kernel)                     \
+     : a->dim <= 64  ? launch(kernel<64>, __VA_ARGS__ Shape<64>::bytes, p, dev.index, st, #kernel)                     \
+     : a->dim <= 128 ? launch(kernel<128>, __VA_ARGS__ Shape<128>::bytes, p, dev.index, st, #kernel)                   \
+                     : launch(kernel<256>, __VA_ARGS__ Shape<256>::bytes, p, dev.index, st, #kernel))
 
 int launch_tc_forward(const rdvb_attention* a, const Params& p, const rdvb_host::Device& dev, cudaStream_t st) {
     const int64_t items = ceil_div(a->q_len, 2 * kTcTile) * a->heads * a->batch * p.splits;
@@ -223,9 +223,8 @@ int launch_tc_forward(const rdvb_attention* a, const Params& p, const rdvb_host:
     if (int rc = encode(&k, a, a->k, a->k_stride, a->kv_len, a->kv_heads)) return rc;
     if (int rc = encode(&v, a, a->v, a->v_stride, a->kv_len, a->kv_heads)) return rc;
     auto go = [&](auto kernel, uint32_t smem) -> int {
-        cudaError_t e =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(smem), dev.index))
+            return rc;
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, dev.sm_count));
         kernel<<<grid, kTcThreads, smem, st>>>(t, static_cast<uint32_t>(items), q, k, v);
         return rdvb_host::launched("tc_forward_kernel");
@@ -257,9 +256,9 @@ int launch_few(const rdvb_attention* a, const Params& p, cudaStream_t st) {
     return rdvb_host::launched("few_kernel");
 }
 
-// dQ, dK and dV of a call that tensor_core() takes; `join` sums parts.
-template <typename Join>
-int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* workspace, cudaStream_t st, Join join) {
+// dQ, dK and dV, or their parts, of a call that tensor_core() takes.
+int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* workspace, const rdvb_host::Device& dev,
+                       cudaStream_t st) {
     GradParams g;
     if (int rc = rdvb_host::status_word(&g.status)) return rc;
     const int64_t stats = static_cast<int64_t>(a->batch) * a->heads * l.q_pad;
@@ -287,14 +286,11 @@ int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* w
     if (int rc = rdvb_host::launched("tc_prep_kernel")) return rc;
     auto go = [&](auto kernel, uint32_t smem, int64_t blocks, const char* what) -> int {
         if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what);
-        cudaError_t e =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(smem), dev.index))
+            return rc;
         kernel<<<static_cast<unsigned>(blocks), kGradThreads, smem, st>>>(g, q, k, v, d);
         return rdvb_host::launched(what);
     };
-    const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
-    const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
     g.a.splits = l.dq;
     g.a.split_len = l.dq_len;
     int64_t blocks = l.q_pad / kTcTile * a->heads * a->batch * l.dq;
@@ -303,22 +299,13 @@ int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* w
                         : (bf16 ? go(tc_dq_kernel<128, true>, TcDq<128>::kBytes, blocks, "tc_dq_kernel")
                                 : go(tc_dq_kernel<128, false>, TcDq<128>::kBytes, blocks, "tc_dq_kernel")))
         return rc;
-    if (l.dq > 1)
-        if (int rc = join(p.part, l.dq, rows * a->dim, rows * a->dim, p.dq)) return rc;
     g.a.splits = l.dkv;
     g.a.split_len = l.dkv_len;
     blocks = ceil_div(a->kv_len, kTcTile) * a->kv_heads * a->batch * l.dkv;
-    if (int rc = narrow ? (bf16 ? go(tc_dkv_kernel<64, true>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel")
-                                : go(tc_dkv_kernel<64, false>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel"))
-                        : (bf16 ? go(tc_dkv_kernel<128, true>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel")
-                                : go(tc_dkv_kernel<128, false>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel")))
-        return rc;
-    if (l.dkv > 1) {
-        const int64_t n = kv_rows * a->dim;
-        if (int rc = join(p.part, l.dkv, 2 * n, n, p.dk)) return rc;
-        if (int rc = join(p.part + n, l.dkv, 2 * n, n, p.dv)) return rc;
-    }
-    return RDVB_OK;
+    return narrow ? (bf16 ? go(tc_dkv_kernel<64, true>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel")
+                          : go(tc_dkv_kernel<64, false>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel"))
+                  : (bf16 ? go(tc_dkv_kernel<128, true>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel")
+                          : go(tc_dkv_kernel<128, false>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel"));
 }
 
 int simple_launch_check(int64_t blocks, const char* what) {
@@ -419,35 +406,37 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     p.dq = dq;
     p.dk = dk;
     p.dv = dv;
-    auto join = [&](const float* part, int splits, int64_t pitch, int64_t n, void* to) -> int {
-        const int wide = n % 4 == 0 && pitch % 4 == 0 && aligned(part, 16);
-        const int64_t blocks = ceil_div(n, wide ? 4 * kThreads : kThreads);
-        if (int rc = simple_launch_check(blocks, "join_kernel")) return rc;
-        join_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(part, splits, pitch, n, wide, to, a->dtype);
-        return rdvb_host::launched("join_kernel");
-    };
-    if (l.tc) return launch_tc_backward(a, l, p, workspace, st, join);
-    const int64_t delta_blocks = ceil_div(rows, kThreads / 32);
-    if (int rc = simple_launch_check(delta_blocks, "delta_kernel")) return rc;
-    delta_kernel<<<static_cast<unsigned>(delta_blocks), kThreads, 0, st>>>(p);
-    if (int rc = rdvb_host::launched("delta_kernel")) return rc;
-    const int tile = tile_of(a, false);
-    p.splits = l.dq;
-    p.split_len = l.dq_len;
-    int64_t blocks = ceil_div(a->q_len, tile) * a->heads * a->batch * p.splits;
-    if (int rc = RDVB_BY_DIM(dq_kernel, kBackwardBytes, blocks, )) return rc;
-    if (p.splits > 1)
-        if (int rc = join(p.part, p.splits, rows * a->dim, rows * a->dim, dq)) return rc;
-    p.splits = l.dkv;
-    p.split_len = l.dkv_len;
-    blocks = ceil_div(a->kv_len, tile) * a->kv_heads * a->batch * p.splits;
-    if (int rc = RDVB_BY_DIM(dkv_kernel, kBackwardBytes, blocks, )) return rc;
-    if (p.splits > 1) {
-        const int64_t n = kv_rows * a->dim;
-        if (int rc = join(p.part, p.splits, 2 * n, n, dk)) return rc;
-        if (int rc = join(p.part + n, p.splits, 2 * n, n, dv)) return rc;
+    p.part_kv = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.delta_bytes + l.dq_bytes);
+    if (l.tc) {
+        if (int rc = launch_tc_backward(a, l, p, workspace, dev, st)) return rc;
+    } else {
+        const int64_t delta_blocks = ceil_div(rows, kThreads / 32);
+        if (int rc = simple_launch_check(delta_blocks, "delta_kernel")) return rc;
+        delta_kernel<<<static_cast<unsigned>(delta_blocks), kThreads, 0, st>>>(p);
+        if (int rc = rdvb_host::launched("delta_kernel")) return rc;
+        const int tile = tile_of(a, false);
+        p.splits = l.dq;
+        p.split_len = l.dq_len;
+        int64_t blocks = ceil_div(a->q_len, tile) * a->heads * a->batch * p.splits;
+        if (int rc = RDVB_BY_DIM(dq_kernel, kBackwardBytes, blocks, )) return rc;
+        p.splits = l.dkv;
+        p.split_len = l.dkv_len;
+        blocks = ceil_div(a->kv_len, tile) * a->kv_heads * a->batch * p.splits;
+        if (int rc = RDVB_BY_DIM(dkv_kernel, kBackwardBytes, blocks, )) return rc;
     }
-    return RDVB_OK;
+    if (l.dq == 1 && l.dkv == 1) return RDVB_OK;
+    const int64_t nq = rows * a->dim, nk = kv_rows * a->dim;
+    Joins j;
+    j.g[0] = {p.part, dq, nq, nq, l.dq > 1 ? l.dq : 0};
+    j.g[1] = {p.part_kv, dk, nk, 2 * nk, l.dkv > 1 ? l.dkv : 0};
+    j.g[2] = {p.part_kv + nk, dv, nk, 2 * nk, l.dkv > 1 ? l.dkv : 0};
+    j.dtype = a->dtype;
+    j.wide = nq % 4 == 0 && nk % 4 == 0;
+    const int64_t most = std::max(l.dq > 1 ? nq : 0, l.dkv > 1 ? nk : 0);
+    const int64_t blocks = ceil_div(most, j.wide ? 4 * kThreads : kThreads);
+    if (int rc = simple_launch_check(blocks, "join_kernel")) return rc;
+    join_kernel<<<dim3(static_cast<unsigned>(blocks), 3), kThreads, 0, st>>>(j);
+    return rdvb_host::launched("join_kernel");
 }
 
 }  // extern "C"

@@ -37,7 +37,8 @@ struct Params {
     void *o, *dq, *dk, *dv;  // dense
     float* lse;              // [batch, heads, q_len]
     float* delta;            // [batch, heads, q_len]
-    float* part;             // partial results of splits
+    float* part;             // partial results of splits: rows of the forward pass, dQ
+    float* part_kv;          // of dK and dV
     float* part_stat;
     const int32_t* lengths;  // may be null
     const uint8_t* mask;     // may be null
@@ -135,10 +136,12 @@ template <int DP>
 __device__ __forceinline__ void tile_dot(const float* a, const float* b, int ty, int tx,
                                          float (&s)[Shape<DP>::kPer][Shape<DP>::kPer]) {
     constexpr int kPer = Shape<DP>::kPer, kRow = Shape<DP>::kRow;
+    // even and odd dimensions' sums side by side: one packed instruction for two products
+    float odd[kPer][kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) s[i][j] = 0.0f;
+        for (int j = 0; j < kPer; ++j) s[i][j] = odd[i][j] = 0.0f;
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
         float4 x[kPer], y[kPer];
@@ -150,12 +153,16 @@ __device__ __forceinline__ void tile_dot(const float* a, const float* b, int ty,
         for (int i = 0; i < kPer; ++i)
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
-                s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-                s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-                s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-                s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+                float p0 = x[i].x, p1 = x[i].y;
+                fma2(p0, p1, y[j].x, y[j].y, s[i][j], odd[i][j]);
+                s[i][j] = x[i].z, odd[i][j] = x[i].w;
+                fma2(s[i][j], odd[i][j], y[j].z, y[j].w, p0, p1);
             }
     }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) s[i][j] += odd[i][j];
 }
 
 // acc[i][j] += sum over n of w[ty + 16 i][n] x[n][out_dim(tx, j)].
@@ -174,12 +181,21 @@ __device__ __forceinline__ void tile_mac(const float* w, const float* x, int ty,
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             float b[kCols];
+            constexpr int kChunk = DP >= 64 ? 4 : 2;
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) b[j] = x[(n + m) * kRow + out_dim<DP>(tx, j)];
+            for (int j = 0; j < kCols; j += kChunk) {
+                const auto v = *reinterpret_cast<const Vec<float, kChunk>*>(x + (n + m) * kRow + out_dim<DP>(tx, j));
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) b[j + i] = v.v[i];
+            }
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) acc[i][j] = fmaf(a[i][m], b[j], acc[i][j]);
+                for (int j = 0; j < kCols; j += 2) {
+                    float p0 = b[j], p1 = b[j + 1];
+                    fma2(p0, p1, a[i][m], a[i][m], acc[i][j], acc[i][j + 1]);
+                    acc[i][j] = p0, acc[i][j + 1] = p1;
+                }
         }
     }
 }
@@ -531,8 +547,8 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const Params p) {
             if (d >= p.dim) continue;
             const float gk = on ? dk[i][j] * p.scale : 0.0f, gv = on ? dv[i][j] : 0.0f;
             if (p.splits > 1) {
-                p.part[(2 * split * rows + row) * p.dim + d] = gk;
-                p.part[((2 * split + 1) * rows + row) * p.dim + d] = gv;
+                p.part_kv[(2 * split * rows + row) * p.dim + d] = gk;
+                p.part_kv[((2 * split + 1) * rows + row) * p.dim + d] = gv;
             } else {
                 store1(p.dk, p.dtype, row * p.dim + d, gk);
                 store1(p.dv, p.dtype, row * p.dim + d, gv);
@@ -541,31 +557,43 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const Params p) {
     }
 }
 
-// Sums `splits` parts of n floats each, `pitch` apart, in split order, four
-// elements a thread where `wide` (n and pitch multiples of 4).
-__global__ void __launch_bounds__(kThreads) join_kernel(const float* part, int splits, int64_t pitch, int64_t n, int wide,
-                                                        void* out, int dtype) {
-    const int64_t i = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) * (wide ? 4 : 1);
-    if (i >= n) return;
-    if (wide) {
+// One gradient's parts: `splits` of n floats each, `pitch` apart; 0 splits:
+// nothing to join.
+struct Join {
+    const float* part;
+    void* out;
+    int64_t n, pitch;
+    int splits;
+};
+struct Joins {
+    Join g[3];  // dQ, dK, dV
+    int dtype;
+    int wide;  // every n and pitch a multiple of 4: four elements a thread
+};
+// Sums the parts in split order. Block y: which gradient.
+__global__ void __launch_bounds__(kThreads) join_kernel(const Joins p) {
+    const Join& g = p.g[blockIdx.y];
+    const int64_t i = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) * (p.wide ? 4 : 1);
+    if (g.splits == 0 || i >= g.n) return;
+    if (p.wide) {
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) {
-            const float4 v = *reinterpret_cast<const float4*>(part + s * pitch + i);
+        for (int s = 0; s < g.splits; ++s) {
+            const float4 v = *reinterpret_cast<const float4*>(g.part + s * g.pitch + i);
             sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
         const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        if (dtype == 0)
-            store_f32<float, 4>(static_cast<float*>(out) + i, v);
-        else if (dtype == 1)
-            store_f32<__half, 4>(static_cast<__half*>(out) + i, v);
+        if (p.dtype == 0)
+            store_f32<float, 4>(static_cast<float*>(g.out) + i, v);
+        else if (p.dtype == 1)
+            store_f32<__half, 4>(static_cast<__half*>(g.out) + i, v);
         else
-            store_f32<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(out) + i, v);
+            store_f32<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(g.out) + i, v);
         return;
     }
     float sum = 0.0f;
-    for (int s = 0; s < splits; ++s) sum += part[s * pitch + i];
-    store1(out, dtype, i, sum);
+    for (int s = 0; s < g.splits; ++s) sum += g.part[s * g.pitch + i];
+    store1(g.out, p.dtype, i, sum);
 }
 
 }  // namespace attn

@@ -527,8 +527,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float c = a.scale * kLog2e;
         uint32_t n = 0;  // key tiles of this query tile so far
         bool ok = true;
+        TcItem next = tc_item(a, blockIdx.x);
         for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const TcItem t = tc_item(a, id);
+            const TcItem t = next;
+            if (id + gridDim.x < items) next = tc_item(a, id + gridDim.x);  // its length is on its way meanwhile
             if (w && !t.both) continue;
             float top = -INFINITY, total = 0.0f;
             bool any = false;

@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         // WG 0 writes dV, WG 1 dK
         const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_len * a.kv_heads;
         const int64_t row = (b * a.kv_len + key) * a.kv_heads + hk;
-        float* part = a.splits > 1 ? a.part + (2 * split + (half ? 0 : 1)) * rows * a.dim : nullptr;
+        float* part = a.splits > 1 ? a.part_kv + (2 * split + (half ? 0 : 1)) * rows * a.dim : nullptr;
         const float f = half ? a.scale * exp2f(-e2) : exp2f(-kP);
 #pragma unroll 1
         for (int d = 0; d < DP; d += 16) {

@@ -24,6 +24,7 @@ int fail_text(int code, const char* text);  // records the calling thread's mess
 int launched(const char* what);             // the launch's error status; counts the launch
 int device(Device* out);                    // refuses a device that is not sm_100
 int status_word(uint32_t** out);            // device address of the status word
+int allow_smem(const void* kernel, int bytes, int device);  // dynamic shared memory, set once a kernel and device
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();  // null when the driver has none
 
 __attribute__((format(printf, 2, 3))) inline int fail(int code, const char* fmt, ...) {

@@ -171,11 +171,7 @@ int rdvb_group_norm(const void* x, int dtype, int64_t n, int64_t rows, int c, in
         if constexpr (kOne) {
             if (status) {
                 auto kernel = small_kernel<T, kVec, kAct>;
-                cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallBytes);
-                if (e != cudaSuccess) {
-                    rc = fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-                    return;
-                }
+                if ((rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), kSmallBytes, dev.index))) return;
                 kernel<<<static_cast<unsigned>(n), kThreads, static_cast<size_t>(sample), st>>>(p, status);
                 rc = rdvb_host::launched("group_norm small_kernel");
                 return;

@@ -12,8 +12,10 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <map>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include "rdvb.h"
 #include "host.h"
@@ -2163,6 +2165,18 @@ int status_word(uint32_t** out) {
         at[dev] = static_cast<uint32_t*>(p);
     }
     *out = at[dev];
+    return RDVB_OK;
+}
+
+int allow_smem(const void* kernel, int bytes, int device) {
+    static std::mutex mutex;
+    static std::map<std::pair<const void*, int>, int> set;
+    std::lock_guard<std::mutex> lock(mutex);
+    int& have = set[{kernel, device}];
+    if (bytes <= have) return RDVB_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    have = bytes;
     return RDVB_OK;
 }
 
