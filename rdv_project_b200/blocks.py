@@ -118,10 +118,15 @@ def group_norm_forward(x, groups: int, weight=None, bias=None, eps: float = 1e-5
     return _group_norm(x, groups, weight, bias, eps, activation, True)
 
 
+def _as_param(grad, param):
+    kind = getattr(param, "dtype", torch.float32)
+    return grad if grad is None or kind not in _DTYPES else grad.to(kind)
+
+
 def group_norm_backward(dy, x, stats, groups: int, weight=None, bias=None, activation=None):
     """(dx, dweight, dbias) of group_norm_forward's y for the gradient dy;
-    dweight and dbias have their parameter's type (float32 sums), None for
-    a parameter that is None."""
+    dweight and dbias have their parameter tensor's type (float32 sums), None
+    for a parameter that is None."""
     x, w, b, kind, n, rows, c = _norm_args(x, groups, weight, bias, activation)
     dy = _tensor(dy).contiguous()
     if not (dy.shape == x.shape and dy.dtype == x.dtype):
@@ -140,8 +145,7 @@ def group_norm_backward(dy, x, stats, groups: int, weight=None, bias=None, activ
             dy.data_ptr(), x.data_ptr(), stats.data_ptr(), _DTYPES[x.dtype], n, rows, c, groups, _ptr(w), _ptr(b),
             kind, _ACTIVATIONS[activation], dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nbytes, stream_handle()),
             "rdvb_group_norm_backward")
-    return (dx, dw if dw is None else dw.to(as_device_tensor(weight).dtype),
-            db if db is None else db.to(as_device_tensor(bias).dtype))
+    return dx, _as_param(dw, weight), _as_param(db, bias)
 
 
 class _GroupNorm(torch.autograd.Function):

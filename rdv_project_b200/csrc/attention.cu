@@ -132,11 +132,12 @@ Plan plan(const rdvb_attention* a) {
     const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
     const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
     // The tensor-core kernels hold one block a processor (the forward one takes two query tiles), the CUDA-core ones
-    // two; a step is a pair of 128 x 128 tiles (measured at about 0.8 and 1.2 us) or of 64 x 64 (about 8 us).
+    // two. Microseconds a step, measured: 128 keys against 256 queries, 128 x 128 for dQ and for dK and dV; 64 x 64.
     const int64_t slots = p.tc ? 148 : 296;
+    const bool narrow = a->dim <= 64;
     const double row_bytes = static_cast<double>(a->dim) * 4;
     p.forward = splits_for((p.tc ? ceil_div(q_tiles, 2) : q_tiles) * a->heads * a->batch, k_tiles, slots,
-                           p.tc ? 1.2 : 8.0, rows * row_bytes);
+                           p.tc ? (narrow ? 1.9 : 2.5) : 12.0, rows * row_bytes);
     p.forward_len = ceil_div(k_tiles, p.forward) * tile;
     p.few = few_rows(a);
     if (p.few) {
@@ -150,11 +151,13 @@ Plan plan(const rdvb_attention* a) {
     p.forward_bytes = p.forward > 1 ? round16(p.forward * rows * 8) + p.forward * rows * a->dim * 4 : 0;
     // gradients
     const int64_t bq_tiles = ceil_div(a->q_len, back), bk_tiles = ceil_div(a->kv_len, back);
-    p.dq = splits_for(bq_tiles * a->heads * a->batch, bk_tiles, slots, p.tc ? 0.8 : 12.0, rows * row_bytes);
+    p.dq = splits_for(bq_tiles * a->heads * a->batch, bk_tiles, slots,
+                      p.tc ? (narrow ? 1.4 : 1.6) : 16.0, rows * row_bytes);
     p.dq_len = ceil_div(bk_tiles, p.dq) * back;
     p.dq = static_cast<int>(std::max<int64_t>(1, ceil_div(a->kv_len, std::max<int64_t>(p.dq_len, 1))));
     const int64_t items = bq_tiles * (a->heads / a->kv_heads);
-    p.dkv = splits_for(bk_tiles * a->kv_heads * a->batch, items, slots, p.tc ? 1.2 : 16.0, 2 * kv_rows * row_bytes);
+    p.dkv = splits_for(bk_tiles * a->kv_heads * a->batch, items, slots,
+                       p.tc ? (narrow ? 1.5 : 2.4) : 16.0, 2 * kv_rows * row_bytes);
     p.dkv_len = ceil_div(items, p.dkv);
     p.dkv = static_cast<int>(std::max<int64_t>(1, ceil_div(items, std::max<int64_t>(p.dkv_len, 1))));
     p.q_pad = bq_tiles * back;

@@ -2171,12 +2171,16 @@ int status_word(uint32_t** out) {
 int allow_smem(const void* kernel, int bytes, int device) {
     static std::mutex mutex;
     static std::map<std::pair<const void*, int>, int> set;
-    std::lock_guard<std::mutex> lock(mutex);
-    int& have = set[{kernel, device}];
-    if (bytes <= have) return RDVB_OK;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    have = bytes;
+    try {
+        std::lock_guard<std::mutex> lock(mutex);
+        int& have = set[{kernel, device}];
+        if (bytes <= have) return RDVB_OK;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return fail(RDVB_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        have = bytes;
+    } catch (...) {  // no memory for the entry
+        return fail(RDVB_ERR_CUDA, "out of host memory");
+    }
     return RDVB_OK;
 }
 
