@@ -190,16 +190,21 @@ __device__ __forceinline__ KeyLoad key_load(const Params& p, int b, int64_t k0, 
         l.m[i] = p.mask && 32 * i + lane < l.left ? p.mask[b * p.mask_stride + k0 + 32 * i + lane] : 0;
     return l;
 }
-__device__ __forceinline__ KeyBits key_bits(const Params& p, const KeyLoad& l) {
+// The first `left` keys.
+__device__ __forceinline__ KeyBits key_range(int left) {
     KeyBits bits;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int n = l.left - 32 * i;
-        if (p.mask)
-            bits.w[i] = __ballot_sync(0xffffffffu, l.m[i] != 0);
-        else
-            bits.w[i] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+        const int n = left - 32 * i;
+        bits.w[i] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
     }
+    return bits;
+}
+__device__ __forceinline__ KeyBits key_bits(const Params& p, const KeyLoad& l) {
+    if (!p.mask) return key_range(l.left);
+    KeyBits bits;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits.w[i] = __ballot_sync(0xffffffffu, l.m[i] != 0);
     return bits;
 }
 
@@ -527,19 +532,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float c = a.scale * kLog2e;
         uint32_t n = 0;  // key tiles of this query tile so far
         bool ok = true;
-        TcItem next = tc_item(a, blockIdx.x);
         for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const TcItem t = next;
-            if (id + gridDim.x < items) next = tc_item(a, id + gridDim.x);  // its length is on its way meanwhile
+            const TcItem t = tc_item(a, id);
             if (w && !t.both) continue;
             float top = -INFINITY, total = 0.0f;
             bool any = false;
             KeyLoad keys = key_load(a, t.b, t.begin, t.end);
             for (int i = 0; i < t.tiles; ++i, ++n) {
-                const KeyBits bits = key_bits(a, keys);
-                keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
-                const bool whole = bits.all();
-                any |= !bits.none();
+                KeyBits bits;
+                bool whole;
+                if (a.mask) {
+                    bits = key_bits(a, keys);
+                    keys = key_load(a, t.b, t.begin + (i + 1) * kTcTile, t.end);
+                    whole = bits.all();
+                    any |= !bits.none();
+                } else {
+                    bits = key_range(t.end - t.begin - i * kTcTile);
+                    whole = i + 1 < t.tiles || (t.end - t.begin) % kTcTile == 0;
+                    any = true;
+                }
                 if (!(ok = mbar_wait_warp(s_full + 8 * w, n & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
                 tc_fence_after();
                 uint32_t r[8][16];
