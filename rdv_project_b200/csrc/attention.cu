@@ -287,28 +287,35 @@ int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* w
         bf16 ? tc_prep_kernel<16, true><<<kPrepBlocks, kThreads, 0, st>>>(g)
              : tc_prep_kernel<16, false><<<kPrepBlocks, kThreads, 0, st>>>(g);
     if (int rc = rdvb_host::launched("tc_prep_kernel")) return rc;
-    auto go = [&](auto kernel, uint32_t smem, int64_t blocks, const char* what) -> int {
-        if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what);
-        if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(smem), dev.index))
-            return rc;
-        kernel<<<static_cast<unsigned>(blocks), kGradThreads, smem, st>>>(g, q, k, v, d);
-        return rdvb_host::launched(what);
-    };
     g.a.splits = l.dq;
     g.a.split_len = l.dq_len;
-    int64_t blocks = l.q_pad / kTcTile * a->heads * a->batch * l.dq;
-    if (int rc = narrow ? (bf16 ? go(tc_dq_kernel<64, true>, TcDq<64>::kBytes, blocks, "tc_dq_kernel")
-                                : go(tc_dq_kernel<64, false>, TcDq<64>::kBytes, blocks, "tc_dq_kernel"))
-                        : (bf16 ? go(tc_dq_kernel<128, true>, TcDq<128>::kBytes, blocks, "tc_dq_kernel")
-                                : go(tc_dq_kernel<128, false>, TcDq<128>::kBytes, blocks, "tc_dq_kernel")))
+    const int64_t items = l.q_pad / kTcTile * a->heads * a->batch * l.dq;
+    if (items > 0x3fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "tc_dq_kernel: too many query tiles");
+    auto go_q = [&](auto kernel, uint32_t smem) -> int {
+        if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(smem), dev.index))
+            return rc;
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(items, dev.sm_count));
+        kernel<<<grid, kGradThreads, smem, st>>>(g, static_cast<uint32_t>(items), q, k, v, d);
+        return rdvb_host::launched("tc_dq_kernel");
+    };
+    if (int rc = narrow ? (bf16 ? go_q(tc_dq_kernel<64, true>, TcDq<64>::kBytes)
+                                : go_q(tc_dq_kernel<64, false>, TcDq<64>::kBytes))
+                        : (bf16 ? go_q(tc_dq_kernel<128, true>, TcDq<128>::kBytes)
+                                : go_q(tc_dq_kernel<128, false>, TcDq<128>::kBytes)))
         return rc;
     g.a.splits = l.dkv;
     g.a.split_len = l.dkv_len;
-    blocks = ceil_div(a->kv_len, kTcTile) * a->kv_heads * a->batch * l.dkv;
-    return narrow ? (bf16 ? go(tc_dkv_kernel<64, true>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel")
-                          : go(tc_dkv_kernel<64, false>, TcDkv<64>::kBytes, blocks, "tc_dkv_kernel"))
-                  : (bf16 ? go(tc_dkv_kernel<128, true>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel")
-                          : go(tc_dkv_kernel<128, false>, TcDkv<128>::kBytes, blocks, "tc_dkv_kernel"));
+    const int64_t blocks = ceil_div(a->kv_len, kTcTile) * a->kv_heads * a->batch * l.dkv;
+    if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "tc_dkv_kernel: too many blocks");
+    auto go = [&](auto kernel, uint32_t smem) -> int {
+        if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(smem), dev.index))
+            return rc;
+        kernel<<<static_cast<unsigned>(blocks), kGradThreads, smem, st>>>(g, q, k, v, d);
+        return rdvb_host::launched("tc_dkv_kernel");
+    };
+    return narrow ? (bf16 ? go(tc_dkv_kernel<64, true>, TcDkv<64>::kBytes) : go(tc_dkv_kernel<64, false>, TcDkv<64>::kBytes))
+                  : (bf16 ? go(tc_dkv_kernel<128, true>, TcDkv<128>::kBytes)
+                          : go(tc_dkv_kernel<128, false>, TcDkv<128>::kBytes));
 }
 
 int simple_launch_check(int64_t blocks, const char* what) {

@@ -225,28 +225,40 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, const KeyBits& bits) {
     }
 }
 
-// A block's place in the forward pass and dQ: query tile, head, sample,
-// split.
-struct TcPlace {
-    int64_t q0, begin, end;
+// An item of the forward pass (two tiles of query rows of one head over the
+// keys of one split) or of dQ (one tile).
+struct TcItem {
+    int q0, begin, end;  // positions fit 31 bits
     int h, hk, b, split, tiles;
+    bool both;  // the second tile has rows
 };
-__device__ __forceinline__ TcPlace tc_place(const Params& p) {
-    TcPlace t;
-    const uint32_t q_tiles = static_cast<uint32_t>((p.q_len + kTcTile - 1) / kTcTile);
-    uint32_t id = blockIdx.x;
-    t.q0 = static_cast<int64_t>(id % q_tiles) * kTcTile;
-    id /= q_tiles;
+template <int kTiles>
+__device__ __forceinline__ TcItem tc_item(const Params& p, uint32_t id) {
+    TcItem t;
+    const uint32_t q_items = static_cast<uint32_t>((p.q_len + kTiles * kTcTile - 1) / (kTiles * kTcTile));
+    t.q0 = static_cast<int>(id % q_items) * (kTiles * kTcTile);
+    id /= q_items;
     t.h = id % p.heads;
     id /= p.heads;
     t.b = id % p.batch;
     t.split = id / p.batch;
     t.hk = t.h / p.group;
-    const int64_t len = length_of(p, t.b);
-    t.begin = t.split * p.split_len;
-    t.end = min(len, t.begin + p.split_len);
-    t.tiles = t.end > t.begin ? static_cast<int>((t.end - t.begin + kTcTile - 1) / kTcTile) : 0;
+    t.both = kTiles == 2 && t.q0 + kTcTile < p.q_len;
+    const int64_t len = length_of(p, t.b), begin = t.split * p.split_len, end = min(len, begin + p.split_len);
+    t.begin = static_cast<int>(begin);
+    t.end = static_cast<int>(end);
+    t.tiles = end > begin ? static_cast<int>((end - begin + kTcTile - 1) / kTcTile) : 0;
     return t;
+}
+
+// The next item of this block with keys, from `id` on; false past the last.
+template <int kTiles>
+__device__ __forceinline__ bool next_item(const Params& p, uint32_t items, uint32_t& id, TcItem& t) {
+    for (; id < items; id += gridDim.x) {
+        t = tc_item<kTiles>(p, id);
+        if (t.tiles > 0) return true;
+    }
+    return false;
 }
 
 // 2^x for x <= 128: x = n + f, |f| <= 1/2, times a polynomial of degree 4 in
@@ -299,40 +311,6 @@ struct TcForward {
     // dimensions the exponential unit is what the products wait for.
     static constexpr int kPoly = DP == 64 ? 1 : 0;
 };
-
-// An item of the forward pass: 256 query rows of one head over the keys of
-// one split.
-struct TcItem {
-    int q0, begin, end;  // positions fit 31 bits
-    int h, hk, b, split, tiles;
-    bool both;  // the second tile has rows
-};
-__device__ __forceinline__ TcItem tc_item(const Params& p, uint32_t id) {
-    TcItem t;
-    const uint32_t q_items = static_cast<uint32_t>((p.q_len + 2 * kTcTile - 1) / (2 * kTcTile));
-    t.q0 = static_cast<int>(id % q_items) * (2 * kTcTile);
-    id /= q_items;
-    t.h = id % p.heads;
-    id /= p.heads;
-    t.b = id % p.batch;
-    t.split = id / p.batch;
-    t.hk = t.h / p.group;
-    t.both = t.q0 + kTcTile < p.q_len;
-    const int64_t len = length_of(p, t.b), begin = t.split * p.split_len, end = min(len, begin + p.split_len);
-    t.begin = static_cast<int>(begin);
-    t.end = static_cast<int>(end);
-    t.tiles = end > begin ? static_cast<int>((end - begin + kTcTile - 1) / kTcTile) : 0;
-    return t;
-}
-
-// The next item of this block with keys, from `id` on; false past the last.
-__device__ __forceinline__ bool next_item(const Params& p, uint32_t items, uint32_t& id, TcItem& t) {
-    for (; id < items; id += gridDim.x) {
-        t = tc_item(p, id);
-        if (t.tiles > 0) return true;
-    }
-    return false;
-}
 
 template <int DP, bool kBf16>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -387,7 +365,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t n = 0, k_sent = 0, v_sent = 0, q_sent = 0, id = blockIdx.x;  // n: key tiles so far
                 TcItem t;
                 bool ok = true;
-                for (; ok && next_item(a, items, id, t); id += gridDim.x) {
+                for (; ok && next_item<2>(a, items, id, t); id += gridDim.x) {
                     if (!mbar_wait(q_empty, (q_sent & 1) ^ 1, abort_flag, p.status, kStatusTimeoutWEmpty)) break;
                     ++q_sent;
                     tc_load<F::kAtoms>(s_q, map_q, t.h, t.q0, t.b, q_full);
@@ -469,13 +447,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 };
                 uint32_t id = blockIdx.x, n = 0, query_items = 0;
                 TcItem t, u;
-                bool ok = true, have = next_item(a, items, id, t);
+                bool ok = true, have = next_item<2>(a, items, id, t);
 #pragma unroll
                 for (int m = 0; m < kMine; ++m)
                     if (ok && have && (w0 + m == 0 || t.both)) ok = score(m, t, 0, 0, 0);
                 while (ok && have) {
                     uint32_t next = id + gridDim.x;  // u: the item after t
-                    const bool more = next_item(a, items, next, u);
+                    const bool more = next_item<2>(a, items, next, u);
                     ++query_items;
                     for (int i = 0; ok && i < t.tiles; ++i, ++n) {
                         const bool within = i + 1 < t.tiles;
@@ -505,7 +483,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t n = 0, id = blockIdx.x;
                 TcItem t;
                 bool ok = true;
-                for (; ok && next_item(a, items, id, t); id += gridDim.x) {
+                for (; ok && next_item<2>(a, items, id, t); id += gridDim.x) {
                     KeyLoad keys = key_load(a, t.b, t.begin, t.end);
                     for (int i = 0; i < t.tiles; ++i, ++n) {
                         const uint32_t s = n % kStages;
@@ -533,7 +511,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t n = 0;  // key tiles of this query tile so far
         bool ok = true;
         for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const TcItem t = tc_item(a, id);
+            const TcItem t = tc_item<2>(a, id);
             if (w && !t.both) continue;
             float top = -INFINITY, total = 0.0f;
             bool any = false;

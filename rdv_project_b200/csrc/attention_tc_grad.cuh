@@ -212,14 +212,16 @@ __device__ __forceinline__ void store_columns(const Params& a, void* out, float*
 
 // ------------------------------------------------------------------------ dQ
 //
-// A block: 128 query rows of one head over the keys of one split. S has two
+// An item: 128 query rows of one head over the keys of one split. S has two
 // buffers (dS(i) replaces S(i)), dP one: S(i + 1) and dP(i + 1) run beside the
-// exponentials of i and dQ(i).
+// exponentials of i and dQ(i). A block stays and takes item after item, with
+// counters that run on from one to the next; up to 64 dimensions Q, dO and dQ
+// have two buffers, so that short key sequences do not wait between items.
 template <int DP>
 struct TcDq {
-    static constexpr int kAtoms = DP / 64, kKStages = 3, kVStages = 2;
+    static constexpr int kAtoms = DP / 64, kKStages = 3, kVStages = 2, kItems = DP == 64 ? 2 : 1;
     static constexpr uint32_t kTileBytes = kTcTile * DP * 2;
-    static constexpr uint32_t kOffDo = kTileBytes, kOffK = 2 * kTileBytes, kOffV = kOffK + kKStages * kTileBytes,
+    static constexpr uint32_t kOffK = 2 * kItems * kTileBytes, kOffV = kOffK + kKStages * kTileBytes,
                               kOffBar = kOffV + kVStages * kTileBytes;
     static constexpr uint32_t kBytes = kOffBar + 256 + 1024;
     static constexpr uint32_t kColS = 0, kColDp = 256, kColDq = 384;
@@ -227,29 +229,33 @@ struct TcDq {
 
 template <int DP, bool kBf16>
 __global__ void __launch_bounds__(kGradThreads, 1)
-    tc_dq_kernel(const GradParams p, const __grid_constant__ TcMap map_q, const __grid_constant__ TcMap map_k,
-                 const __grid_constant__ TcMap map_v, const __grid_constant__ TcMap map_do) {
+    tc_dq_kernel(const GradParams p, const uint32_t items, const __grid_constant__ TcMap map_q,
+                 const __grid_constant__ TcMap map_k, const __grid_constant__ TcMap map_v,
+                 const __grid_constant__ TcMap map_do) {
     using F = TcDq<DP>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t s_q = base, s_do = base + F::kOffDo, s_k = base + F::kOffK, s_v = base + F::kOffV,
-                   bars = base + F::kOffBar;
-    const uint32_t q_full = bars, dp_full = bars + 8, drain = bars + 16, s_full = bars + 24, ds_full = bars + 40,
-                   dq_done = bars + 56, k_tma = bars + 72, k_ok = bars + 96, k_empty = bars + 120,
-                   v_full = bars + 144, v_empty = bars + 160;
-    const uint32_t tmem_slot = bars + 176;
+    const uint32_t s_q = base, s_k = base + F::kOffK, s_v = base + F::kOffV, bars = base + F::kOffBar;
+    // by item (even and odd where there are two buffers), by key tile, by stage
+    const uint32_t q_full = bars, q_empty = bars + 16, dq_full = bars + 32, dq_read = bars + 48, dp_full = bars + 64,
+                   drain = bars + 72, s_full = bars + 80, ds_full = bars + 96, dq_done = bars + 112,
+                   k_tma = bars + 128, k_ok = bars + 152, k_empty = bars + 176, v_full = bars + 200,
+                   v_empty = bars + 216;
+    const uint32_t tmem_slot = bars + 232;
     volatile uint32_t* abort_flag =
-        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 180);
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 236);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Params& a = p.a;
-    const TcPlace t = tc_place(a);
 
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
-        mbar_init(q_full, 2);  // Q and dO
         mbar_init(dp_full, 1);
         mbar_init(drain, 2);  // an arrival an issuing warp
         for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full + 8 * i, 2);  // Q and dO
+            mbar_init(q_empty + 8 * i, 1);
+            mbar_init(dq_full + 8 * i, 1);
+            mbar_init(dq_read + 8 * i, 8);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(ds_full + 8 * i, 8);
             mbar_init(dq_done + 8 * i, 1);
@@ -271,176 +277,231 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
 
     if (warp == 8) {
-        if (lane == 0 && t.tiles > 0) {
-            int k_sent = 0, v_sent = 0;
-            tc_load<F::kAtoms>(s_q, map_q, t.h, t.q0, t.b, q_full);
-            tc_load<F::kAtoms>(s_do, map_do, t.h, t.q0, t.b, q_full);
-            for (int i = 0; i < t.tiles; ++i) {
-                const int sk = i % F::kKStages, sv = i % F::kVStages;
-                const int64_t k0 = t.begin + static_cast<int64_t>(i) * kTcTile;
-                if (!mbar_wait(k_empty + 8 * sk, ((i / F::kKStages) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutXEmpty))
+        if (lane == 0) {
+            uint32_t n = 0, m = 0, k_sent = 0, v_sent = 0, id = blockIdx.x;  // n: key tiles, m: items so far
+            TcItem t;
+            bool ok = true;
+            for (; ok && next_item<1>(a, items, id, t); id += gridDim.x) {
+                const uint32_t slot = m % F::kItems;
+                if (!mbar_wait(q_empty + 8 * slot, ((m / F::kItems) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutWEmpty))
                     break;
-                tc_load<F::kAtoms>(s_k + sk * F::kTileBytes, map_k, t.hk, k0, t.b, k_tma + 8 * sk);
-                ++k_sent;
-                if (!mbar_wait(v_empty + 8 * sv, ((i / F::kVStages) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutXEmpty))
-                    break;
-                tc_load<F::kAtoms>(s_v + sv * F::kTileBytes, map_v, t.hk, k0, t.b, v_full + 8 * sv);
-                ++v_sent;
+                ++m;
+                tc_load<F::kAtoms>(s_q + 2 * slot * F::kTileBytes, map_q, t.h, t.q0, t.b, q_full + 8 * slot);
+                tc_load<F::kAtoms>(s_q + (2 * slot + 1) * F::kTileBytes, map_do, t.h, t.q0, t.b, q_full + 8 * slot);
+                for (int i = 0; i < t.tiles; ++i, ++n) {
+                    const uint32_t sk = n % F::kKStages, sv = n % F::kVStages;
+                    const int64_t k0 = t.begin + static_cast<int64_t>(i) * kTcTile;
+                    ok = mbar_wait(k_empty + 8 * sk, ((n / F::kKStages) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutXEmpty);
+                    if (!ok) break;
+                    tc_load<F::kAtoms>(s_k + sk * F::kTileBytes, map_k, t.hk, k0, t.b, k_tma + 8 * sk);
+                    ++k_sent;
+                    ok = mbar_wait(v_empty + 8 * sv, ((n / F::kVStages) & 1) ^ 1, abort_flag, p.status, kStatusTimeoutXEmpty);
+                    if (!ok) break;
+                    tc_load<F::kAtoms>(s_v + sv * F::kTileBytes, map_v, t.hk, k0, t.b, v_full + 8 * sv);
+                    ++v_sent;
+                }
             }
-            drain_wait(q_full, 0, p.status);
-            for (int s = 0; s < F::kKStages; ++s)
+            // no copy may be in flight when the block ends
+            for (uint32_t s = 0; s < F::kItems; ++s)
+                if (m > s) drain_wait(q_full + 8 * s, ((m - 1 - s) / F::kItems) & 1, p.status);
+            for (uint32_t s = 0; s < F::kKStages; ++s)
                 if (k_sent > s) drain_wait(k_tma + 8 * s, ((k_sent - 1 - s) / F::kKStages) & 1, p.status);
-            for (int s = 0; s < F::kVStages; ++s)
+            for (uint32_t s = 0; s < F::kVStages; ++s)
                 if (v_sent > s) drain_wait(v_full + 8 * s, ((v_sent - 1 - s) / F::kVStages) & 1, p.status);
         }
     } else if (warp == 9) {
-        if (lane == 0 && t.tiles > 0) {
+        if (lane == 0) {
             const uint32_t idesc = umma_idesc_f16(kTcTile, kBf16);
             const uint32_t k_ready = p.guarded ? k_ok : k_tma;
-            const uint32_t q_desc = desc_k_major(s_q), do_desc = desc_k_major(s_do), k_desc = desc_k_major(s_k),
-                           v_desc = desc_k_major(s_v);
-            auto score = [&](int i) {  // S(i), over dS(i - 2)
-                const uint32_t s = i % F::kKStages, half = i & 1;
-                if (i >= 2 &&
-                    !mbar_wait(dq_done + 8 * half, (i / 2 - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull))
+            const uint32_t q_desc = desc_k_major(s_q), k_desc = desc_k_major(s_k), v_desc = desc_k_major(s_v);
+            constexpr uint32_t kTile = F::kTileBytes / 16;
+            auto score = [&](uint32_t n, uint32_t m, bool first) {  // S(n) of item m, over dS(n - 2)
+                const uint32_t s = n % F::kKStages, half = n & 1, slot = m % F::kItems;
+                if (first &&
+                    !mbar_wait(q_full + 8 * slot, (m / F::kItems) & 1, abort_flag, p.status, kStatusTimeoutWFull))
                     return false;
-                if (!mbar_wait(k_ready + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                if (n >= 2 &&
+                    !mbar_wait(dq_done + 8 * half, (n / 2 - 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull))
+                    return false;
+                if (!mbar_wait(k_ready + 8 * s, (n / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows<DP / 16>(tmem + F::kColS + half * 128, q_desc, k_desc + s * (F::kTileBytes / 16), p.k_steps,
-                                      idesc);
+                product_rows<DP / 16>(tmem + F::kColS + half * 128, q_desc + 2 * slot * kTile, k_desc + s * kTile,
+                                      p.k_steps, idesc);
                 umma_commit(s_full + 8 * half);
                 return true;
             };
-            auto reach = [&](int i) {  // dP(i), over dP(i - 1), which was read before dS(i - 1) was complete
-                const uint32_t s = i % F::kVStages;
-                if (i >= 1 && !mbar_wait(ds_full + 8 * ((i - 1) & 1), ((i - 1) / 2) & 1, abort_flag, p.status,
+            auto reach = [&](uint32_t n, uint32_t m, bool last) {  // dP(n), over dP(n - 1), which dS(n - 1) was made of
+                const uint32_t s = n % F::kVStages, slot = m % F::kItems;
+                if (n >= 1 && !mbar_wait(ds_full + 8 * ((n - 1) & 1), ((n - 1) / 2) & 1, abort_flag, p.status,
                                          kStatusTimeoutAFull))
                     return false;
-                if (!mbar_wait(v_full + 8 * s, (i / F::kVStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
+                if (!mbar_wait(v_full + 8 * s, (n / F::kVStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
                     return false;
                 tc_fence_after();
-                product_rows<DP / 16>(tmem + F::kColDp, do_desc, v_desc + s * (F::kTileBytes / 16), p.k_steps, idesc);
+                product_rows<DP / 16>(tmem + F::kColDp, q_desc + (2 * slot + 1) * kTile, v_desc + s * kTile, p.k_steps,
+                                      idesc);
                 umma_commit(v_empty + 8 * s);
                 umma_commit(dp_full);
+                if (last) umma_commit(q_empty + 8 * slot);
                 return true;
             };
-            bool ok = mbar_wait(q_full, 0, abort_flag, p.status, kStatusTimeoutWFull) && score(0);
-            for (int i = 0; ok && i < t.tiles; ++i) {
-                ok = reach(i);
-                if (ok && i + 1 < t.tiles) ok = score(i + 1);
+            uint32_t id = blockIdx.x, n = 0;
+            TcItem t;
+            bool ok = true, have = next_item<1>(a, items, id, t);
+            if (have) ok = score(0, 0, true);
+            for (uint32_t m = 0; ok && have; ++m) {
+                const int tiles = t.tiles;
+                id += gridDim.x;
+                have = next_item<1>(a, items, id, t);
+                for (int i = 0; ok && i < tiles; ++i, ++n) {
+                    const bool last = i + 1 == tiles;
+                    ok = reach(n, m, last);
+                    if (ok && (!last || have)) ok = score(n + 1, last ? m + 1 : m, last);
+                }
             }
             umma_commit(drain);
             drain_wait(drain, 0, p.status);
         }
     } else if (warp == 11) {
-        if (lane == 0 && t.tiles > 0) {
+        if (lane == 0) {
             const uint32_t idesc = umma_idesc_f16(p.n_pv, kBf16) | kIdescBTransposed;
             const uint32_t k_desc = desc_mn_major(s_k);
-            for (int i = 0; i < t.tiles; ++i) {
-                const uint32_t s = i % F::kKStages, half = i & 1;
-                if (!mbar_wait(ds_full + 8 * half, (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull)) break;
-                tc_fence_after();
-                product_columns(tmem + F::kColDq, tmem + F::kColS + half * 128, k_desc + s * (F::kTileBytes / 16), idesc,
-                                i == 0);
-                umma_commit(k_empty + 8 * s);
-                umma_commit(dq_done + 8 * half);
+            uint32_t id = blockIdx.x, n = 0;
+            TcItem t;
+            bool ok = true;
+            for (uint32_t m = 0; ok && next_item<1>(a, items, id, t); id += gridDim.x, ++m) {
+                const uint32_t slot = m % F::kItems;
+                if (m >= F::kItems && !mbar_wait(dq_read + 8 * slot, (m / F::kItems - 1) & 1, abort_flag, p.status,
+                                                 kStatusTimeoutDrain))
+                    break;
+                for (int i = 0; i < t.tiles; ++i, ++n) {
+                    const uint32_t s = n % F::kKStages, half = n & 1;
+                    ok = mbar_wait(ds_full + 8 * half, (n / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull);
+                    if (!ok) break;
+                    tc_fence_after();
+                    product_columns(tmem + F::kColDq + slot * DP, tmem + F::kColS + half * 128,
+                                    k_desc + s * (F::kTileBytes / 16), idesc, i == 0);
+                    umma_commit(k_empty + 8 * s);
+                    umma_commit(dq_done + 8 * half);
+                }
+                if (ok) umma_commit(dq_full + 8 * slot);
             }
             umma_commit(drain);
             drain_wait(drain, 0, p.status);
         }
     } else if (warp == 10) {
         if (p.guarded) {
-            KeyLoad keys = key_load(a, t.b, t.begin, t.end);
-            for (int i = 0; i < t.tiles; ++i) {
-                const int s = i % F::kKStages;
-                const KeyBits bits = key_bits(a, keys);
-                keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
-                if (!mbar_wait_warp(k_tma + 8 * s, (i / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull))
-                    break;
-                if (!bits.all()) {
-                    zero_rows<F::kAtoms>(s_k + s * F::kTileBytes, bits);
-                    fence_proxy_async_smem();
-                    __syncwarp();
+            uint32_t n = 0, id = blockIdx.x;
+            TcItem t;
+            bool ok = true;
+            for (; ok && next_item<1>(a, items, id, t); id += gridDim.x) {
+                KeyLoad keys = key_load(a, t.b, t.begin, t.end);
+                for (int i = 0; i < t.tiles; ++i, ++n) {
+                    const uint32_t s = n % F::kKStages;
+                    const KeyBits bits = key_bits(a, keys);
+                    keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
+                    ok = mbar_wait_warp(k_tma + 8 * s, (n / F::kKStages) & 1, abort_flag, p.status, kStatusTimeoutXFull);
+                    if (!ok) break;
+                    if (!bits.all()) {
+                        zero_rows<F::kAtoms>(s_k + s * F::kTileBytes, bits);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(k_ok + 8 * s);
                 }
-                if (lane == 0) mbar_arrive(k_ok + 8 * s);
             }
         }
-    } else if (warp < 8) {
+    } else {
         const int half = warp >> 2;
         const uint32_t row_base = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-        const int64_t q = t.q0 + (warp & 3) * 32 + lane;
         const float c = a.scale * kLog2e;
         const float e2 = grad_exponent<kBf16>(p);
-        const int64_t stat = (static_cast<int64_t>(t.b) * a.heads + t.h) * p.q_pad + q;
-        const float minus = p.neg_lse[stat] + e2, neg_delta = p.neg_delta[stat];
-        bool ok = true, any = false;
-        KeyLoad keys = key_load(a, t.b, t.begin, t.end);
-        for (int i = 0; i < t.tiles; ++i) {
-            const KeyBits bits = key_bits(a, keys);
-            keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
-            const bool whole = bits.all();
-            any |= !bits.none();
-            const uint32_t s_col = row_base + F::kColS + (i & 1) * 128 + half * 64;
-            if (!(ok = mbar_wait_warp(s_full + 8 * (i & 1), (i >> 1) & 1, abort_flag, p.status, kStatusTimeoutAccFull)))
-                break;
-            tc_fence_after();
-            uint32_t r[2][32];
-            tmem_ld32(s_col, r[0]);
-            tmem_ld32(s_col + 32, r[1]);
-            tmem_wait_ld32(r[0]);
-            reg_barrier32(r[1]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
-                    fma2(x, y, c, c, minus, minus);
-                    exp2_pair<kGradPoly>(x, y, e / 2);
-                    r[j][e] = __float_as_uint(x);
-                    r[j][e + 1] = __float_as_uint(y);
-                }
-            if (!(ok = mbar_wait_warp(dp_full, i & 1, abort_flag, p.status, kStatusTimeoutAccFull))) break;
-            tc_fence_after();
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t d[32], packed[16];
-                tmem_ld32(row_base + F::kColDp + half * 64 + 32 * j, d);
-                tmem_wait_ld32(d);
-                const uint32_t word = half ? bits.w[2 + j] : bits.w[j];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x = __uint_as_float(d[e]), y = __uint_as_float(d[e + 1]);
-                    add2(x, y, neg_delta, neg_delta);
-                    mul2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
-                    if (!whole) {
-                        x = word >> e & 1u ? x : 0.0f;
-                        y = word >> (e + 1) & 1u ? y : 0.0f;
-                    }
-                    packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
-                }
-                tmem_st16(s_col + 16 * j, packed);
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full + 8 * (i & 1));
-        }
-        if (t.tiles > 0 && ok) ok = mbar_wait_warp(drain, 0, abort_flag, p.status, kStatusTimeoutAccFull);
-        tc_fence_after();
-        const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;
-        const int64_t row = (t.b * a.q_len + q) * a.heads + t.h;
-        float* part = a.splits > 1 ? a.part + t.split * rows * a.dim : nullptr;
         const float f = a.scale * exp2f(-e2);
-#pragma unroll 1
-        for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 16) {
-            if (d >= a.dim) break;
-            uint32_t r[16] = {};
-            if (t.tiles > 0) {
-                tmem_ld16(row_base + F::kColDq + d, r);
-                tmem_wait_ld(r);
+        const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;
+        uint32_t n = 0, m = 0;
+        bool ok = true;
+        for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+            const TcItem t = tc_item<1>(a, id);
+            const int64_t q = t.q0 + (warp & 3) * 32 + lane;
+            const int64_t stat = (static_cast<int64_t>(t.b) * a.heads + t.h) * p.q_pad + q;
+            const float minus = p.neg_lse[stat] + e2, neg_delta = p.neg_delta[stat];
+            bool any = false;
+            KeyLoad keys = key_load(a, t.b, t.begin, t.end);
+            for (int i = 0; i < t.tiles; ++i, ++n) {
+                const KeyBits bits = key_bits(a, keys);
+                keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
+                const bool whole = bits.all();
+                any |= !bits.none();
+                const uint32_t s_col = row_base + F::kColS + (n & 1) * 128 + half * 64;
+                ok = mbar_wait_warp(s_full + 8 * (n & 1), (n / 2) & 1, abort_flag, p.status, kStatusTimeoutAccFull);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t r[2][32];
+                tmem_ld32(s_col, r[0]);
+                tmem_ld32(s_col + 32, r[1]);
+                tmem_wait_ld32(r[0]);
+                reg_barrier32(r[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
+                        fma2(x, y, c, c, minus, minus);
+                        exp2_pair<kGradPoly>(x, y, e / 2);
+                        r[j][e] = __float_as_uint(x);
+                        r[j][e + 1] = __float_as_uint(y);
+                    }
+                ok = mbar_wait_warp(dp_full, n & 1, abort_flag, p.status, kStatusTimeoutAccFull);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t d[32], packed[16];
+                    tmem_ld32(row_base + F::kColDp + half * 64 + 32 * j, d);
+                    tmem_wait_ld32(d);
+                    const uint32_t word = half ? bits.w[2 + j] : bits.w[j];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float x = __uint_as_float(d[e]), y = __uint_as_float(d[e + 1]);
+                        add2(x, y, neg_delta, neg_delta);
+                        mul2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
+                        if (!whole) {
+                            x = word >> e & 1u ? x : 0.0f;
+                            y = word >> (e + 1) & 1u ? y : 0.0f;
+                        }
+                        packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                    }
+                    tmem_st16(s_col + 16 * j, packed);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_full + 8 * (n & 1));
             }
-            if (ok && q < a.q_len) store_columns<kBf16>(a, a.dq, part, row * a.dim, d, r, f, any);
+            const uint32_t slot = m % F::kItems;
+            if (t.tiles > 0 && ok)
+                ok = mbar_wait_warp(dq_full + 8 * slot, (m / F::kItems) & 1, abort_flag, p.status, kStatusTimeoutAccFull);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t row = (t.b * a.q_len + q) * a.heads + t.h;
+            float* part = a.splits > 1 ? a.part + t.split * rows * a.dim : nullptr;
+#pragma unroll 1
+            for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 16) {
+                if (d >= a.dim) break;
+                uint32_t r[16] = {};
+                if (t.tiles > 0) {
+                    tmem_ld16(row_base + F::kColDq + slot * DP + d, r);
+                    tmem_wait_ld(r);
+                }
+                if (q < a.q_len) store_columns<kBf16>(a, a.dq, part, row * a.dim, d, r, f, any);
+            }
+            if (t.tiles > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(dq_read + 8 * slot);
+                ++m;
+            }
         }
     }
     tc_fence_before();
