@@ -39,15 +39,14 @@ struct GradParams {
     int guarded;
 };
 
-// neg_lse, neg_delta and norms: kLanes lanes a row of 16 bytes each, in
-// memory order, four rows of dO and O in flight a thread. Bound: memory.
+// neg_lse, neg_delta and norms: kLanes lanes a row of 16 bytes each, four
+// rows of dO and O in flight a thread. A warp takes consecutive positions of
+// one head, so that what it writes lies together. Bound: memory.
 template <int kLanes, bool kBf16>
 __global__ void __launch_bounds__(kThreads) tc_prep_kernel(const GradParams p) {
-    constexpr int kFlight = 4;
+    constexpr int kFlight = 4, kGroups = 32 / kLanes, kChunk = kFlight * kGroups;  // rows of a warp's step
     const Params& a = p.a;
-    const int sub = threadIdx.x % kLanes;
-    const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / kLanes;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kLanes);
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, group = lane / kLanes;
     auto load8 = [&](const void* src, int64_t at, float (&v)[8]) {
         if (kBf16)
             load_f32<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16*>(src) + at, v);
@@ -55,19 +54,23 @@ __global__ void __launch_bounds__(kThreads) tc_prep_kernel(const GradParams p) {
             load_f32<__half, 8>(static_cast<const __half*>(src) + at, v);
     };
     const bool in = sub * 8 < a.dim;
-    const uint32_t heads = a.heads, length = static_cast<uint32_t>(a.q_len);
-    const int64_t rows = static_cast<int64_t>(a.batch) * length * heads;
-    const int64_t rounds = (rows + step * kFlight - 1) / (step * kFlight);  // the same for every lane of a warp
+    const uint32_t per_head = static_cast<uint32_t>(p.q_pad / kChunk);
+    const int64_t chunks = static_cast<int64_t>(a.batch) * a.heads * per_head;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
     float most_do = 0.0f, most_v = 0.0f;
-    for (int64_t i = 0; i < rounds; ++i) {
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads / 32) + threadIdx.x / 32; i < chunks; i += warps) {
+        const int64_t head = i / per_head, q0 = (i - head * per_head) * kChunk + group;  // of all samples' heads
+        const int64_t b = head / a.heads, h = head - b * a.heads;
         uint4 raw_o[kFlight], raw_g[kFlight];
 #pragma unroll
         for (int j = 0; j < kFlight; ++j) {
-            const int64_t row = first + (i * kFlight + j) * step;
-            const bool real = row < rows && in;
-            const int64_t at = row * a.dim + sub * 8;
-            raw_o[j] = real ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + at)) : make_uint4(0, 0, 0, 0);
-            raw_g[j] = real ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dout) + at)) : make_uint4(0, 0, 0, 0);
+            const int64_t q = q0 + j * kGroups;
+            const int64_t at = ((b * a.q_len + q) * a.heads + h) * a.dim + sub * 8;
+            raw_o[j] = raw_g[j] = make_uint4(0, 0, 0, 0);
+            if (q < a.q_len && in) {
+                raw_o[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.out) + at));
+                raw_g[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dout) + at));
+            }
         }
 #pragma unroll
         for (int j = 0; j < kFlight; ++j) {
@@ -84,35 +87,17 @@ __global__ void __launch_bounds__(kThreads) tc_prep_kernel(const GradParams p) {
                 dot += __shfl_xor_sync(0xffffffffu, dot, e);
                 if (!kBf16) norm += __shfl_xor_sync(0xffffffffu, norm, e);
             }
-            const int64_t row = first + (i * kFlight + j) * step;
-            if (row < rows && sub == 0) {
-                uint32_t q, h, b;
-                if (rows < 0x100000000LL) {  // 32-bit divisions where they do
-                    const uint32_t r = static_cast<uint32_t>(row);
-                    q = r / heads, h = r - q * heads, b = q / length;
-                    q -= b * length;
-                } else {
-                    h = static_cast<uint32_t>(row % heads);
-                    q = static_cast<uint32_t>(row / heads % length);
-                    b = static_cast<uint32_t>(row / heads / length);
-                }
-                const int64_t head = static_cast<int64_t>(b) * heads + h;
-                p.neg_delta[head * p.q_pad + q] = -dot;
-                p.neg_lse[head * p.q_pad + q] = -a.lse[head * length + q] * kLog2e;
+            const int64_t q = q0 + j * kGroups;
+            if (sub == 0) {
+                p.neg_delta[head * p.q_pad + q] = -dot;  // 0 past the end
+                p.neg_lse[head * p.q_pad + q] = q < a.q_len ? -a.lse[head * a.q_len + q] * kLog2e : -INFINITY;
             }
             if (!kBf16) most_do = fmaxf(most_do, norm);
         }
     }
-    // past the end of a head's rows, up to whole tiles
-    const int64_t gap = p.q_pad - a.q_len;
-    const int64_t gaps = gap * a.batch * heads;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < gaps;
-         i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t at = i / gap * p.q_pad + a.q_len + i % gap;
-        p.neg_delta[at] = 0.0f;
-        p.neg_lse[at] = -INFINITY;
-    }
     if (kBf16) return;
+    const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / kLanes;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kLanes);
     const int64_t v_rows = static_cast<int64_t>(a.batch) * a.kv_len * a.kv_heads;
     const int64_t v_rounds = (v_rows + step - 1) / step;
     for (int64_t i = 0; i < v_rounds; ++i) {
