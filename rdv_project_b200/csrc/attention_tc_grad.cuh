@@ -18,6 +18,7 @@
 // that gradients keep their digits whatever the loss was scaled by.
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
 #include "attention_tc.cuh"
 
@@ -202,13 +203,20 @@ __device__ __forceinline__ void store_columns(const Params& a, void* out, float*
 // exponentials of i and dQ(i). A block stays and takes item after item, with
 // counters that run on from one to the next; up to 64 dimensions Q, dO and dQ
 // have two buffers, so that short key sequences do not wait between items.
+//
+// delta = rowsum(dO O) comes from the rounded O, which shows where few keys
+// matter: dP - delta is then a small difference (of one key: 0). Its exact
+// value is sum P dP. Where a row's keys are one tile, dS is made with that;
+// where they are several, the sum of dS, which should be 0, is what delta was
+// off by, and the kernel of dK and dV after this one gets delta with it.
 template <int DP>
 struct TcDq {
     static constexpr int kAtoms = DP / 64, kKStages = 3, kVStages = 2, kItems = DP == 64 ? 2 : 1;
     static constexpr uint32_t kTileBytes = kTcTile * DP * 2;
     static constexpr uint32_t kOffK = 2 * kItems * kTileBytes, kOffV = kOffK + kKStages * kTileBytes,
                               kOffBar = kOffV + kVStages * kTileBytes;
-    static constexpr uint32_t kBytes = kOffBar + 256 + 1024;
+    static constexpr uint32_t kOffRow = kOffBar + 512;  // a float a half row: sums exchanged by a row's two threads
+    static constexpr uint32_t kBytes = kOffRow + 1024 + 1024;
     static constexpr uint32_t kColS = 0, kColDp = 256, kColDq = 384;
 };
 
@@ -226,7 +234,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                    drain = bars + 72, s_full = bars + 80, ds_full = bars + 96, dq_done = bars + 112,
                    k_tma = bars + 128, k_ok = bars + 152, k_empty = bars + 176, v_full = bars + 200,
                    v_empty = bars + 216;
-    const uint32_t tmem_slot = bars + 232;
+    const uint32_t tmem_slot = bars + 232, row_pair = bars + 240;
     volatile uint32_t* abort_flag =
         reinterpret_cast<volatile uint32_t*>(smem_raw + (bars - smem_addr(smem_raw)) + 236);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -234,6 +242,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
+        for (int i = 0; i < 4; ++i) mbar_init(row_pair + 8 * i, 2);
         mbar_init(dp_full, 1);
         mbar_init(drain, 2);  // an arrival an issuing warp
         for (int i = 0; i < 2; ++i) {
@@ -402,15 +411,34 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const uint32_t row_base = tmem + (static_cast<uint32_t>(warp & 3) << 21);
         const float c = a.scale * kLog2e;
         const float e2 = grad_exponent<kBf16>(p);
-        const float f = a.scale * exp2f(-e2);
+        const float to_p = exp2f(-e2), f = a.scale * to_p;
         const int64_t rows = static_cast<int64_t>(a.batch) * a.q_len * a.heads;
-        uint32_t n = 0, m = 0;
+        uint32_t n = 0, m = 0, pair_phase = 0;
         bool ok = true;
+        // v summed over the two threads of a row (warps w and w + 4); false when the wait ran out
+        const uint32_t pair = row_pair + 8 * (warp & 3), cell = base + F::kOffRow + ((warp & 3) * 32 + lane) * 4;
+        auto row_sum = [&](float& v) {
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(cell + half * 512), "f"(v) : "memory");
+            for (int step = 0; step < 2; ++step) {  // written by both; read by both
+                __syncwarp();
+                if (lane == 0) mbar_arrive(pair);
+                if (!mbar_wait_warp(pair, pair_phase++ & 1, abort_flag, p.status, kStatusTimeoutOther)) return false;
+                if (step == 0) {
+                    float other;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(cell + (half ^ 1) * 512) : "memory");
+                    v = half ? other + v : v + other;
+                }
+            }
+            return true;
+        };
         for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const TcItem t = tc_item<1>(a, id);
+            const bool one = t.tiles == 1 && a.splits == 1;
+            float slip0 = 0.0f, slip1 = 0.0f;  // sum of dS
             const int64_t q = t.q0 + (warp & 3) * 32 + lane;
             const int64_t stat = (static_cast<int64_t>(t.b) * a.heads + t.h) * p.q_pad + q;
-            const float minus = p.neg_lse[stat] + e2, neg_delta = p.neg_delta[stat];
+            const float minus = p.neg_lse[stat] + e2;
+            float neg_delta = p.neg_delta[stat];
             bool any = false;
             KeyLoad keys = key_load(a, t.b, t.begin, t.end);
             for (int i = 0; i < t.tiles; ++i, ++n) {
@@ -440,29 +468,68 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 ok = mbar_wait_warp(dp_full, n & 1, abort_flag, p.status, kStatusTimeoutAccFull);
                 if (!ok) break;
                 tc_fence_after();
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t d[32], packed[16];
-                    tmem_ld32(row_base + F::kColDp + half * 64 + 32 * j, d);
-                    tmem_wait_ld32(d);
-                    const uint32_t word = half ? bits.w[2 + j] : bits.w[j];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float x = __uint_as_float(d[e]), y = __uint_as_float(d[e + 1]);
-                        add2(x, y, neg_delta, neg_delta);
-                        mul2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
-                        if (!whole) {
+                uint32_t d[2][32];
+                tmem_ld32(row_base + F::kColDp + half * 64, d[0]);
+                tmem_ld32(row_base + F::kColDp + half * 64 + 32, d[1]);
+                tmem_wait_ld32(d[0]);
+                reg_barrier32(d[1]);
+                // Two copies of the arithmetic: selecting what is not allowed away costs a tenth where all are.
+                auto finish = [&](auto masked) {
+                    constexpr bool kMasked = decltype(masked)::value;
+                    auto keep = [&](float& x, float& y, uint32_t word, int e) {
+                        if (kMasked) {  // whatever stood where the key is not allowed
                             x = word >> e & 1u ? x : 0.0f;
                             y = word >> (e + 1) & 1u ? y : 0.0f;
                         }
-                        packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                    };
+                    if (one) {
+                        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t word = half ? bits.w[2 + j] : bits.w[j];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                float x = __uint_as_float(r[j][e]), y = __uint_as_float(r[j][e + 1]);
+                                mul2(x, y, __uint_as_float(d[j][e]), __uint_as_float(d[j][e + 1]));
+                                keep(x, y, word, e);
+                                add2(s0, s1, x, y);
+                            }
+                        }
+                        s0 += s1;
+                        if (!row_sum(s0)) return false;
+                        neg_delta = -s0 * to_p;
                     }
-                    tmem_st16(s_col + 16 * j, packed);
-                }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t packed[16];
+                        const uint32_t word = half ? bits.w[2 + j] : bits.w[j];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float x = __uint_as_float(d[j][e]), y = __uint_as_float(d[j][e + 1]);
+                            add2(x, y, neg_delta, neg_delta);
+                            mul2(x, y, __uint_as_float(r[j][e]), __uint_as_float(r[j][e + 1]));
+                            keep(x, y, word, e);
+                            add2(slip0, slip1, x, y);
+                            packed[e / 2] = kBf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                        }
+                        tmem_st16(s_col + 16 * j, packed);
+                    }
+                    return true;
+                };
+                ok = whole ? finish(std::false_type{}) : finish(std::true_type{});
+                if (!ok) break;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_full + 8 * (n & 1));
+            }
+            if (t.tiles > 0 && ok && a.splits == 1) {
+                if (!one) {
+                    slip0 += slip1;
+                    ok = row_sum(slip0);
+                    neg_delta -= slip0 * to_p;
+                }
+                if (ok && half == 0 && any && q < a.q_len) p.neg_delta[stat] = neg_delta;
             }
             const uint32_t slot = m % F::kItems;
             if (t.tiles > 0 && ok)

@@ -333,6 +333,36 @@ def test_attention_small_gradients(rdv, cuda_device, dtype):
             near(got, exact[name][0], dtype, exact[name][1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lk", [1, 2, 5, 100])
+@pytest.mark.parametrize("d", [40, 64, 128])
+def test_attention_few_keys_gradients(rdv, cuda_device, dtype, lk, d):
+    """Where few keys matter dP - delta is a small difference. Of keys within one
+    tile delta is exact: dS's error is its own rounding, u |dS|, and float32's of
+    what it is the difference of -- not that of the rounded output."""
+    q, k, v, dout = inputs(lk + d, 2, 150, lk, 4, 2, d, dtype)
+    lengths = [lk, (lk + 1) // 2]
+    keep, scale = keep_of(k, lengths, None), d ** -0.5
+    exact, lse64 = attend64(q, k, v, keep, scale, dout)
+    out, lse = rdv.cross_attention_forward(q, k, v, lengths=lengths)
+    dq, dk, _ = rdv.cross_attention_backward(dout, q, k, v, out, lse, lengths=lengths)
+    zero = torch.zeros((), dtype=torch.float64, device=cuda_device)
+    qd, do = q.double().permute(0, 2, 1, 3), dout.double().permute(0, 2, 1, 3)
+    kd, vd = (torch.where(keep[:, :, None, None], t.double(), zero).permute(0, 2, 1, 3).repeat_interleave(2, 1)
+              for t in (k, v))
+    s = torch.where(keep[:, None, None], qd @ kd.transpose(-1, -2) * scale, -math.inf)
+    p = torch.softmax(s, -1)
+    ds = p * (do @ vd.transpose(-1, -2) - (do * (p @ vd)).sum(-1, keepdim=True)) * scale
+    own_q = ds.abs() @ kd.abs()
+    own_k = (ds.abs().transpose(-1, -2) @ qd.abs()).reshape(2, 2, 2, lk, d).sum(2)
+    u = U[dtype]
+    for name, got, own in (("dq", dq, own_q), ("dk", dk, own_k)):
+        bound = u * exact[name][0].abs() + u * own.permute(0, 2, 1, 3) + 64 * 2.0 ** -24 * exact[name][1]
+        bound = bound + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        worst = ((got.double() - exact[name][0]).abs() / bound.clamp(min=1e-300)).max().item()
+        assert worst <= 1.0, (name, worst)
+
+
 def test_attention_strides_and_streams(rdv, cuda_device):
     g = gen(21)
     kv = randn(g, 2, 150, 2, 4, 64, dtype=torch.bfloat16)
