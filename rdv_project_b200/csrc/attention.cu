@@ -100,7 +100,7 @@ int tile_of(const rdvb_attention* a, bool tc) { return tc ? kTcTile : a->dim > 1
 // Parts that the long axis is split into: those that make the launch
 // shortest. `blocks` blocks of `steps` loop steps run `slots` at a time, a
 // step takes step_us; parts are written and read once more by a join
-// (part_bytes each, at 6.5 TB/s, and 4 us of launch). At least two steps a
+// (part_bytes each, at 3 TB/s with their launches' ends, and 4 us of launch). At least two steps a
 // part, at most 32 parts.
 int splits_for(int64_t blocks, int64_t steps, int64_t slots, double step_us, double part_bytes) {
     int best = 1;
@@ -108,7 +108,7 @@ int splits_for(int64_t blocks, int64_t steps, int64_t slots, double step_us, dou
     for (int s = 1; s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
         const double rounds = static_cast<double>(ceil_div(blocks * s, slots));
         const double us = rounds * static_cast<double>(ceil_div(steps, s)) * step_us +
-                          (s > 1 ? 4.0 + 2.0 * s * part_bytes / 6.5e6 : 0.0);
+                          (s > 1 ? 4.0 + 2.0 * s * part_bytes / 3e6 : 0.0);
         if (s == 1 || us < 0.97 * least) {
             best = s;
             least = us;
@@ -443,7 +443,7 @@ int rdvb_attention_backward(const rdvb_attention* a, const void* dout, const voi
     j.dtype = a->dtype;
     j.wide = nq % 4 == 0 && nk % 4 == 0;
     const int64_t most = std::max(l.dq > 1 ? nq : 0, l.dkv > 1 ? nk : 0);
-    const int64_t blocks = ceil_div(most, j.wide ? 4 * kThreads : kThreads);
+    const int64_t blocks = ceil_div(most, 4 * (j.wide ? 4 * kThreads : kThreads));
     if (int rc = simple_launch_check(blocks, "join_kernel")) return rc;
     join_kernel<<<dim3(static_cast<unsigned>(blocks), 3), kThreads, 0, st>>>(j);
     return rdvb_host::launched("join_kernel");

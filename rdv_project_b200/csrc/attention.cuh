@@ -570,30 +570,41 @@ struct Joins {
     int dtype;
     int wide;  // every n and pitch a multiple of 4: four elements a thread
 };
-// Sums the parts in split order. Block y: which gradient.
+// Sums the parts in split order. Block y: which gradient. A thread has four
+// places (of four elements each where `wide`) in flight.
 __global__ void __launch_bounds__(kThreads) join_kernel(const Joins p) {
+    constexpr int kFlight = 4;
     const Join& g = p.g[blockIdx.y];
-    const int64_t i = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) * (p.wide ? 4 : 1);
-    if (g.splits == 0 || i >= g.n) return;
-    if (p.wide) {
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int s = 0; s < g.splits; ++s) {
-            const float4 v = *reinterpret_cast<const float4*>(g.part + s * g.pitch + i);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    if (g.splits == 0) return;
+    const int width = p.wide ? 4 : 1;
+    const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads) * kFlight + threadIdx.x) * width;
+    float sum[kFlight][4] = {};
+    for (int s = 0; s < g.splits; ++s) {
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            const int64_t i = first + static_cast<int64_t>(f) * kThreads * width;
+            if (i >= g.n) break;
+            if (p.wide) {
+                const float4 v = __ldcs(reinterpret_cast<const float4*>(g.part + s * g.pitch + i));
+                sum[f][0] += v.x, sum[f][1] += v.y, sum[f][2] += v.z, sum[f][3] += v.w;
+            } else {
+                sum[f][0] += g.part[s * g.pitch + i];
+            }
         }
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        if (p.dtype == 0)
-            store_f32<float, 4>(static_cast<float*>(g.out) + i, v);
-        else if (p.dtype == 1)
-            store_f32<__half, 4>(static_cast<__half*>(g.out) + i, v);
-        else
-            store_f32<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(g.out) + i, v);
-        return;
     }
-    float sum = 0.0f;
-    for (int s = 0; s < g.splits; ++s) sum += g.part[s * g.pitch + i];
-    store1(g.out, p.dtype, i, sum);
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+        const int64_t i = first + static_cast<int64_t>(f) * kThreads * width;
+        if (i >= g.n) break;
+        if (!p.wide)
+            store1(g.out, p.dtype, i, sum[f][0]);
+        else if (p.dtype == 0)
+            store_f32<float, 4>(static_cast<float*>(g.out) + i, sum[f]);
+        else if (p.dtype == 1)
+            store_f32<__half, 4>(static_cast<__half*>(g.out) + i, sum[f]);
+        else
+            store_f32<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(g.out) + i, sum[f]);
+    }
 }
 
 }  // namespace attn
