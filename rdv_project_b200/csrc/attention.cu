@@ -241,22 +241,26 @@ int launch_tc_forward(const rdvb_attention* a, const Params& p, const rdvb_host:
 }
 
 template <typename T>
-int launch_few(const rdvb_attention* a, const Params& p, cudaStream_t st) {
+int launch_few(const rdvb_attention* a, const Params& p, const rdvb_host::Device& dev, cudaStream_t st) {
     const int64_t blocks = static_cast<int64_t>(a->batch) * a->kv_heads * p.splits;
     if (blocks > 0x7fffffffLL) return fail(RDVB_ERR_UNSUPPORTED, "few_kernel: too many blocks");
     const int64_t rows = a->q_len * (a->heads / a->kv_heads), lanes = a->dim / static_cast<int>(16 / sizeof(T));
-    auto go = [&](auto n) {
-        constexpr int kLanes = decltype(n)::value;
-        const unsigned grid = static_cast<unsigned>(blocks);
-        if (rows <= 1) few_kernel<T, kLanes, 1><<<grid, kFewThreads, 0, st>>>(p);
-        else if (rows <= 2) few_kernel<T, kLanes, 2><<<grid, kFewThreads, 0, st>>>(p);
-        else if (rows <= 4) few_kernel<T, kLanes, 4><<<grid, kFewThreads, 0, st>>>(p);
-        else few_kernel<T, kLanes, 8><<<grid, kFewThreads, 0, st>>>(p);
+    auto run = [&](auto kernel, int smem) -> int {
+        if (int rc = rdvb_host::allow_smem(reinterpret_cast<const void*>(kernel), smem, dev.index)) return rc;
+        kernel<<<static_cast<unsigned>(blocks), kFewThreads, smem, st>>>(p);
+        return rdvb_host::launched("few_kernel");
     };
-    if (lanes <= 8) go(std::integral_constant<int, 8>{});
-    else if (lanes <= 16) go(std::integral_constant<int, 16>{});
-    else if constexpr (sizeof(T) == 4) go(std::integral_constant<int, 32>{});
-    return rdvb_host::launched("few_kernel");
+    auto go = [&](auto n) -> int {
+        constexpr int kLanes = decltype(n)::value;
+        if (rows <= 1) return run(few_kernel<T, kLanes, 1>, Few<T, kLanes, 1>::kBytes);
+        if (rows <= 2) return run(few_kernel<T, kLanes, 2>, Few<T, kLanes, 2>::kBytes);
+        if (rows <= 4) return run(few_kernel<T, kLanes, 4>, Few<T, kLanes, 4>::kBytes);
+        return run(few_kernel<T, kLanes, 8>, Few<T, kLanes, 8>::kBytes);
+    };
+    if (lanes <= 8) return go(std::integral_constant<int, 8>{});
+    if constexpr (sizeof(T) == 4)
+        if (lanes > 16) return go(std::integral_constant<int, 32>{});
+    return go(std::integral_constant<int, 16>{});
 }
 
 // dQ, dK and dV, or their parts, of a call that tensor_core() takes.
@@ -358,9 +362,9 @@ int rdvb_attention_forward(const rdvb_attention* a, void* out, float* lse, void*
     p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + round16(p.splits * rows * 8));
     const int64_t blocks = ceil_div(a->q_len, tile_of(a, l.tc)) * a->heads * a->batch * p.splits;
     if (l.few) {
-        const int rc = a->dtype == RDVB_F32   ? launch_few<float>(a, p, st)
-                       : a->dtype == RDVB_F16 ? launch_few<__half>(a, p, st)
-                                              : launch_few<__nv_bfloat16>(a, p, st);
+        const int rc = a->dtype == RDVB_F32   ? launch_few<float>(a, p, dev, st)
+                       : a->dtype == RDVB_F16 ? launch_few<__half>(a, p, dev, st)
+                                              : launch_few<__nv_bfloat16>(a, p, dev, st);
         if (rc) return rc;
     } else if (l.tc) {
         if (int rc = launch_tc_forward(a, p, dev, st)) return rc;

@@ -4,12 +4,14 @@
 //
 // Bound: memory -- each key and value is used for at most eight rows, so the
 // FMA pipe keeps up with HBM and tensor cores would not be faster. A key's
-// dimensions lie along a group of lanes, 16 bytes each; a warp holds kUnroll
-// keys a group in flight, K and V at once, straight from global memory to
-// registers. Partial products of kUnroll keys are summed over the lanes in
-// one exchange that leaves each lane one key's score. Every group of lanes
-// keeps its own maximum, sum and output row; groups are joined at the end in
-// order, blocks (splits of the keys) by join_forward_kernel.
+// dimensions lie along a group of lanes, 16 bytes each; a warp's step is
+// kUnroll keys a group, K and V at once, copied to shared memory by the lanes
+// that read them, kStages steps in flight beside the sums of the oldest; no
+// lane reads what another copied, so there is no barrier. Partial products of
+// kUnroll keys are summed over the lanes in one exchange that leaves each lane
+// one key's score. Every group of lanes keeps its own maximum, sum and output
+// row; groups are joined at the end in order, blocks (splits of the keys) by
+// join_forward_kernel.
 #pragma once
 #include <cstdint>
 
@@ -31,14 +33,25 @@ __device__ __forceinline__ void fma_f32x2_acc(float& c0, float& c1, float a0, fl
 template <typename T, int kLanes, int kRows>
 struct Few {
     static constexpr int kVec = 16 / sizeof(T);            // dimensions a lane
-    static constexpr int kUnroll = kRows > 4 ? 4 : 8;      // keys of a group in flight
+    static constexpr int kUnroll = kRows > 4 ? 4 : 8;      // keys of a group's step
     static constexpr int kGroups = 32 / kLanes;            // groups of a warp
     static constexpr int kBlock = kGroups * kUnroll;       // keys of a warp's step
+    static constexpr int kStages = kRows > 4 ? 4 : 2;      // steps of a warp in flight
+    static constexpr int kStage = 2 * kUnroll * 32;        // pieces of 16 bytes: a lane's of each key, then value
+    static constexpr int kBytes = kFewWarps * kStages * kStage * 16;
 };
 
-// Registers for three blocks a processor up to four rows: their loads hide
-// one another's sums (100003 states, 4 samples, 16 heads of 128 over 4, float16:
-// 198 us; two blocks of 215 registers 234 us, four of half the keys 258 us).
+// 16 bytes to shared memory while the thread goes on; zeros, and nothing read, where !ok.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
+    const int bytes = ok ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+// Registers and stages for three blocks a processor up to four rows (100003
+// states, 4 samples, 16 heads of 128 over 4, float16, with the join: 171 us, 4.8
+// TB/s; two blocks with three stages 185 us, steps of four keys in three blocks
+// with four stages 191 us, in four with three 195 us; loads straight to registers,
+// which wait for the sums, 211 us).
 template <typename T, int kLanes, int kRows>
 __global__ void __launch_bounds__(kFewThreads, kRows > 4 ? 2 : 3) few_kernel(const Params p) {
     using F = Few<T, kLanes, kRows>;
@@ -81,31 +94,59 @@ __global__ void __launch_bounds__(kFewThreads, kRows > 4 ? 2 : 3) few_kernel(con
     for (int i = 0, half = kLanes / 2; (1 << i) < kU; ++i, half /= 2) mine |= (sub & half ? 1 : 0) << i;
     bool any = false;
 
-    for (int64_t k0 = begin + warp * F::kBlock; k0 < end; k0 += kFewWarps * F::kBlock) {
-        Vec<T, kVec> kv[kU], vv[kU];
+    // A lane reads only the pieces that it copied, so its own waits are all that the stages need.
+    extern __shared__ uint4 few_stages[];
+    uint4* const stages = few_stages + warp * F::kStages * F::kStage + lane;
+    const uint32_t stages_at = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
+    constexpr int64_t kStep = kFewWarps * F::kBlock;
+    // Which of the keys of the step from k0 this group may read.
+    auto allowed = [&](int64_t k0) -> uint32_t {
         uint32_t on = 0;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int64_t key = k0 + u * F::kGroups + group;
-            const bool ok = key < end && (!mask || mask[key] != 0);
-            on |= static_cast<uint32_t>(ok) << u;
-            // a key that is not allowed is not read: zeros stand for it
-            uint4 zk = make_uint4(0, 0, 0, 0), zv = zk;
-            if (ok && in) {
-                zk = __ldg(reinterpret_cast<const uint4*>(k_base + key * p.ks.pos));
-                zv = __ldg(reinterpret_cast<const uint4*>(v_base + key * p.vs.pos));
-            }
-            kv[u] = *reinterpret_cast<Vec<T, kVec>*>(&zk);
-            vv[u] = *reinterpret_cast<Vec<T, kVec>*>(&zv);
+            on |= static_cast<uint32_t>(key < end && (!mask || mask[key] != 0)) << u;
         }
-        if (!__any_sync(0xffffffffu, on != 0)) continue;
+        return on;
+    };
+    // A key that is not allowed is not read: zeros stand for it.
+    auto fetch = [&](int64_t k0, uint32_t on, int stage) {
+        if (k0 < end) {
+            const int64_t key = k0 + group;
+            const T *k = k_base + key * p.ks.pos, *v = v_base + key * p.vs.pos;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const bool ok = in && (on >> u & 1u);
+                const uint32_t to = stages_at + (stage * F::kStage + u * 32) * 16;
+                copy16(to, ok ? k + u * F::kGroups * p.ks.pos : k_base, ok);
+                copy16(to + kU * 512, ok ? v + u * F::kGroups * p.vs.pos : v_base, ok);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int64_t k0 = begin + warp * F::kBlock;
+    uint32_t queue = 0;  // the allowed keys of the steps in flight, the oldest lowest
+#pragma unroll
+    for (int i = 0; i < F::kStages; ++i) {
+        const uint32_t on = allowed(k0 + i * kStep);
+        fetch(k0 + i * kStep, on, i);
+        queue |= on << i * kU;
+    }
+    for (int stage = 0; k0 < end; k0 += kStep, stage = stage + 1 == F::kStages ? 0 : stage + 1) {
+        const uint32_t on = queue & ((1u << kU) - 1), later = allowed(k0 + F::kStages * kStep);
+        queue = queue >> kU | later << (F::kStages - 1) * kU;
+        asm volatile("cp.async.wait_group %0;" ::"n"(F::kStages - 1) : "memory");
+        if (!__any_sync(0xffffffffu, on != 0)) {
+            fetch(k0 + F::kStages * kStep, later, stage);
+            continue;
+        }
         any |= on != 0;
+        const uint4* at = stages + stage * F::kStage;
         float s[kU][kRows];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             float x[kVec];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) x[i] = to_f32<T>(kv[u].v[i]);
+            load_f32<T, kVec>(reinterpret_cast<const T*>(at + u * 32), x);
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
                 float s0 = q[r][0] * x[0], s1 = q[r][1] * x[1];
@@ -152,8 +193,7 @@ __global__ void __launch_bounds__(kFewThreads, kRows > 4 ? 2 : 3) few_kernel(con
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             float x[kVec];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) x[i] = to_f32<T>(vv[u].v[i]);
+            load_f32<T, kVec>(reinterpret_cast<const T*>(at + (kU + u) * 32), x);
             // the lane of this group that holds key u
             int from = 0;
 #pragma unroll
@@ -166,6 +206,7 @@ __global__ void __launch_bounds__(kFewThreads, kRows > 4 ? 2 : 3) few_kernel(con
                 for (int i = 0; i < kVec; i += 2) fma_f32x2_acc(acc[r][i], acc[r][i + 1], e, e, x[i], x[i + 1]);
             }
         }
+        fetch(k0 + F::kStages * kStep, later, stage);
     }
 
     // Joins the block's groups, in order.
