@@ -2,16 +2,16 @@
 // eight rows share a key head (positions times query heads a key head), as
 // when a position at a time is served. Every element type.
 //
-// Bound: memory -- each key and value is used for at most eight rows, so the
-// FMA pipe keeps up with HBM and tensor cores would not be faster. A key's
-// dimensions lie along a group of lanes, 16 bytes each; a warp's step is
-// kUnroll keys a group, K and V at once, copied to shared memory by the lanes
-// that read them, kStages steps in flight beside the sums of the oldest; no
-// lane reads what another copied, so there is no barrier. Partial products of
-// kUnroll keys are summed over the lanes in one exchange that leaves each lane
-// one key's score. Every group of lanes keeps its own maximum, sum and output
-// row; groups are joined at the end in order, blocks (splits of the keys) by
-// join_forward_kernel.
+// Bound: memory up to two rows (5.8 TB/s); at four the conversions, sums and
+// exchanges of a key's rows in three warps a scheduler (4.4 TB/s: 0.63 of the
+// issue slots, 57 % of DRAM). A key's dimensions lie along a group of lanes, 16
+// bytes each; a warp's step is kUnroll keys a group, K and V at once, copied to
+// shared memory by the lanes that read them, kStages steps in flight beside the
+// sums of the oldest; no lane reads what another copied, so there is no barrier.
+// Partial products of kUnroll keys are summed over the lanes in one exchange
+// that leaves each lane one key's score. Every group of lanes keeps its own
+// maximum, sum and output row; groups are joined at the end in order, blocks
+// (splits of the keys) by join_forward_kernel.
 #pragma once
 #include <cstdint>
 
@@ -48,10 +48,11 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
 }
 
 // Registers and stages for three blocks a processor up to four rows (100003
-// states, 4 samples, 16 heads of 128 over 4, float16, with the join: 171 us, 4.8
-// TB/s; two blocks with three stages 185 us, steps of four keys in three blocks
-// with four stages 191 us, in four with three 195 us; loads straight to registers,
-// which wait for the sums, 211 us).
+// states, 4 samples, 16 heads of 128 over 4, float16, with the join: 188 us over
+// inputs in turn. Over one input again, whose end is still in L2: 171 us; two
+// blocks with three stages 185 us, steps of four keys in three blocks with four
+// stages 191 us, in four with three 195 us; loads straight to registers, which
+// wait for the sums, 211 us).
 template <typename T, int kLanes, int kRows>
 __global__ void __launch_bounds__(kFewThreads, kRows > 4 ? 2 : 3) few_kernel(const Params p) {
     using F = Few<T, kLanes, kRows>;
