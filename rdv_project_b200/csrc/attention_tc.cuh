@@ -402,8 +402,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         } else if (warp == 9 || (warp == 11 && F::kIssuers == 2)) {
             if (lane == 0) {
-                // Products of query tile w: of both, or of this warp's own. Where an item has no second tile the
-                // first one's releases count twice.
+                // Products of query tile w: of both, or of this warp's own. A barrier that is told apart by parity
+                // must not move on by two phases behind a warp that waits on it. So the second tile's own issuer
+                // goes through every item: where one has no second tile it waits for what it would have read and
+                // releases that at once, and no phase ends without it. A single issuer's releases count twice there.
                 const int w0 = F::kIssuers == 2 && warp == 11 ? 1 : 0;
                 constexpr int kMine = F::kIssuers == 2 ? 1 : 2;
                 const uint32_t idesc_s = umma_idesc_f16(kTcTile, kBf16);
@@ -416,13 +418,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 };
                 auto release = [&](uint32_t bar, bool both) {
                     umma_commit(bar);
-                    if (!both) umma_commit(bar);
+                    if (F::kIssuers == 1 && !both) umma_commit(bar);
                 };
+                // Whether item v has this warp's m-th tile. With an issuer a tile, the functions below are called for
+                // every item; with one, for the tiles that there are.
+                auto has = [&](int m, const TcItem& v) { return w0 + m == 0 || v.both; };
+                auto takes = [&](int m, const TcItem& v) { return F::kIssuers == 2 || has(m, v); };
                 // S of key tile i (the block's n-th) of item v, its query_item-th
                 auto score = [&](int m, const TcItem& v, int i, uint32_t n, uint32_t query_item) {
                     const uint32_t s = n % kStages, w = w0 + m;
                     if (i == 0 && m == 0 && !wait(q_full, query_item, kStatusTimeoutWFull)) return false;
                     if (m == 0 && !wait(k_full + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
+                    if (!has(m, v)) {
+                        mbar_arrive(k_empty + 8 * s);
+                        if (i == v.tiles - 1) mbar_arrive(q_empty);
+                        return true;
+                    }
                     // the softmax has read the last scores, and P does not lie over them or was taken
                     if (scores[m] > 0 &&
                         !wait((F::kOwnP ? s_read : o_full) + 8 * w, scores[m] - 1, kStatusTimeoutAccFull))
@@ -440,6 +451,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 auto mix = [&](int m, const TcItem& v, int i, uint32_t n, uint32_t mixes) {
                     const uint32_t s = n % kStages, w = w0 + m;
                     if (m == 0 && !wait(v_ready + 8 * s, n / kStages, kStatusTimeoutXFull)) return false;
+                    if (!has(m, v)) {
+                        mbar_arrive(v_empty + 8 * s);
+                        return true;
+                    }
                     if (i == 0 && begun[m]++ > 0 && !wait(o_read + 8 * w, begun[m] - 2, kStatusTimeoutDrain))
                         return false;
                     if (!wait(p_full + 8 * w, mixes, kStatusTimeoutAFull)) return false;
@@ -457,7 +472,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 bool ok = true, have = next_item<2>(a, items, id, t);
 #pragma unroll
                 for (int m = 0; m < kMine; ++m)
-                    if (ok && have && (w0 + m == 0 || t.both)) ok = score(m, t, 0, 0, 0);
+                    if (ok && have && takes(m, t)) ok = score(m, t, 0, 0, 0);
                 while (ok && have) {
                     uint32_t next = id + gridDim.x;  // u: the item after t
                     const bool more = next_item<2>(a, items, next, u);
@@ -466,8 +481,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const bool within = i + 1 < t.tiles;
 #pragma unroll
                         for (int m = 0; m < kMine; ++m) {
-                            const bool here = w0 + m == 0 || t.both;
-                            const bool ahead = within ? here : more && (w0 + m == 0 || u.both);
+                            const bool here = takes(m, t);
+                            const bool ahead = within ? here : more && takes(m, u);
                             const uint32_t mixes = scores[m] - 1;
                             if (F::kOwnP && ok && ahead)
                                 ok = within ? score(m, t, i + 1, n + 1, query_items - 1)

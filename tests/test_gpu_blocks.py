@@ -292,6 +292,35 @@ def test_attention_masks_and_poison(rdv, cuda_device, dtype, lq, d):
         assert torch.equal(out, clean) and all(torch.equal(a, e) for a, e in zip(grads, clean_grads))
 
 
+# b, lq, lk, heads, kv_heads, d: more items (two query tiles of a head in the forward pass, one for dQ) than processors,
+# so that a block takes several; last items of one tile and of two, one to nine key tiles
+WALKS = [(8, 577, 400, 8, 8, 64), (8, 576, 1000, 8, 8, 64), (8, 600, 100, 8, 4, 64), (4, 1089, 500, 16, 16, 64),
+         (6, 1100, 260, 16, 4, 64), (2, 2700, 1100, 8, 8, 32), (6, 640, 300, 16, 16, 40), (8, 577, 400, 8, 8, 128),
+         (6, 1300, 300, 8, 2, 128), (10, 500, 150, 8, 8, 72)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("shape", WALKS)
+def test_attention_blocks_take_several_items(rdv, cuda_device, dtype, ragged, shape):
+    """What a block carries from one item to the next: barriers' phases, both
+    buffers of queries, the look-ahead, and samples without states between others."""
+    b, lq, lk, h = shape[:4]
+    processors = torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    assert -(-lq // 256) * h * b > processors
+    q, k, v, dout = inputs(sum(shape) + ragged, *shape, dtype)
+    lengths = mask = None
+    if ragged:
+        lengths = torch.tensor(([lk, 0, lk // 2, 0, 0, 1, lk - 1, 0, 129, lk])[:b], dtype=torch.int32, device=cuda_device)
+        mask = torch.rand(b, lk, generator=gen(lk), device=cuda_device) < 0.8
+        mask[2:3] = False  # a sample whose mask leaves nothing
+    out, grads = check_attention(rdv, q, k, v, dout, lengths, mask)
+    again, lse = rdv.cross_attention_forward(q, k, v, lengths=lengths, mask=mask)
+    grads_again = rdv.cross_attention_backward(dout, q, k, v, again, lse, lengths=lengths, mask=mask)
+    assert torch.equal(again, out) and all(torch.equal(a, e) for a, e in zip(grads_again, grads))
+    assert rdv.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_extreme_scores(rdv, cuda_device, dtype):
     """Scores far apart (one key takes all), equal scores, and scales of both
