@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 bool whole;
                 if (a.mask) {
                     bits = key_bits(a, keys);
-                    keys = key_load(a, t.b, t.begin + (i + 1) * kTcTile, t.end);
+                    keys = key_load(a, t.b, t.begin + (i + 1ll) * kTcTile, t.end);
                     whole = bits.all();
                     any |= !bits.none();
                 } else {

@@ -441,6 +441,22 @@ def test_attention_long_offsets(rdv, cuda_device):
         near(rdv.cross_attention(q, k, v, mask=mask), exact[0], torch.float16, exact[1])
 
 
+def test_attention_last_positions(rdv, cuda_device):
+    """As many states as a call takes, masked: the position after the last tile does
+    not fit 31 bits. Only the end is attended to (34 GB of states, 2 GB of mask)."""
+    lk, d = 2 ** 31 - 1, 8
+    k = torch.zeros(1, lk, 1, d, dtype=torch.float16, device=cuda_device)
+    g = gen(6)
+    k[:, -500:] = randn(g, 1, 500, 1, d, dtype=torch.float16)
+    mask = torch.zeros(1, lk, dtype=torch.bool, device=cuda_device)
+    mask[:, -500:] = torch.rand(500, generator=g, device=cuda_device) < 0.8
+    q = randn(g, 1, 40, 1, d, dtype=torch.float16)
+    out = rdv.cross_attention(q, k, k, mask=mask)
+    end, keep = k[:, -500:], mask[:, -500:]
+    exact = attend64(q, end, end, keep, d ** -0.5)[0]["out"]
+    near(out, exact[0], torch.float16, exact[1])
+
+
 def test_attention_differences_and_repeats(rdv, cuda_device):
     q, k, v, dout = inputs(31, 2, 65, 130, 4, 2, 24, torch.float32)
     lengths = [130, 37]
