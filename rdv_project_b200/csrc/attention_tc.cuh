@@ -636,6 +636,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
             for (int j = 0; j < a.dim; j += 16) {
                 uint32_t r[16] = {};
+                __syncwarp();  // the load takes the whole warp; lanes past q_len skipped the last store
                 if (t.tiles > 0) {
                     tmem_ld16(col_o + j, r);
                     tmem_wait_ld(r);

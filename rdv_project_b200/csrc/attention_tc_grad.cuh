@@ -545,6 +545,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
             for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 16) {
                 if (d >= a.dim) break;
                 uint32_t r[16] = {};
+                __syncwarp();  // the load takes the whole warp; lanes past q_len skipped the last store
                 if (t.tiles > 0) {
                     tmem_ld16(row_base + F::kColDq + slot * DP + d, r);
                     tmem_wait_ld(r);
@@ -803,6 +804,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(dp_read);
+                __syncwarp();  // the stores below take the whole warp
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -839,6 +841,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         for (int d = 0; d < DP; d += 16) {
             if (d >= a.dim) break;
             uint32_t r[16] = {};
+            __syncwarp();  // the load takes the whole warp; lanes past kv_len skipped the last store
             if (items > 0) {
                 tmem_ld16(row_base + (half ? F::kColDk : F::kColDv) + d, r);
                 tmem_wait_ld(r);

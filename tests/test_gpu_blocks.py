@@ -321,6 +321,23 @@ def test_attention_blocks_take_several_items(rdv, cuda_device, dtype, ragged, sh
     assert rdv.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [40, 64, 128])
+@pytest.mark.parametrize("lk", [130, 1500])
+def test_attention_ends_inside_a_warp(rdv, cuda_device, dtype, d, lk):
+    """Rows end inside a warp's 32, positions and states alike: what lanes past the
+    end skip changes nothing of the others' rows, whether parts are joined or not."""
+    q, k, v, dout = inputs(d + lk, 1, 256, lk, 2, 1, d, dtype)
+    dout[:, 129:] = 0
+    for lq in (129, 145, 159, 255):
+        out, grads = check_attention(rdv, q[:, :lq].contiguous(), k, v, dout[:, :lq].contiguous())
+        if lq == 129:
+            first, first_grads = out, grads
+        assert torch.equal(out[:, :129], first) and torch.equal(grads[0][:, :129], first_grads[0])
+    for end in (lk - 1, lk - 17):
+        check_attention(rdv, q, k[:, :end], v[:, :end], dout)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_extreme_scores(rdv, cuda_device, dtype):
     """Scores far apart (one key takes all), equal scores, and scales of both
