@@ -161,8 +161,8 @@ Plan plan(const rdvb_attention* a) {
     p.dkv_len = ceil_div(items, p.dkv);
     p.dkv = static_cast<int>(std::max<int64_t>(1, ceil_div(items, std::max<int64_t>(p.dkv_len, 1))));
     p.q_pad = bq_tiles * back;
-    p.delta_bytes = p.tc ? 2 * static_cast<int64_t>(a->batch) * a->heads * p.q_pad * 4 + kPrepBlocks * 8
-                         : round16(rows * 4);
+    const int64_t stat_bytes = static_cast<int64_t>(a->batch) * a->heads * p.q_pad * 4;
+    p.delta_bytes = p.tc ? (2 + (p.dq > 1 ? p.dq : 0)) * stat_bytes + kPrepBlocks * 8 : round16(rows * 4);
     const int64_t dq_bytes = p.dq > 1 ? p.dq * rows * a->dim * 4 : 0;
     const int64_t dkv_bytes = p.dkv > 1 ? 2 * p.dkv * kv_rows * a->dim * 4 : 0;
     p.dq_bytes = round16(dq_bytes);
@@ -263,6 +263,10 @@ int launch_few(const rdvb_attention* a, const Params& p, const rdvb_host::Device
     return go(std::integral_constant<int, 16>{});
 }
 
+int simple_launch_check(int64_t blocks, const char* what) {
+    return blocks > 0x7fffffffLL ? fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what) : RDVB_OK;
+}
+
 // dQ, dK and dV, or their parts, of a call that tensor_core() takes.
 int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* workspace, const rdvb_host::Device& dev,
                        cudaStream_t st) {
@@ -272,6 +276,7 @@ int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* w
     g.neg_lse = static_cast<float*>(workspace);
     g.neg_delta = g.neg_lse + stats;
     g.norms = reinterpret_cast<float2*>(g.neg_delta + stats);
+    g.slips = reinterpret_cast<float*>(g.norms + kPrepBlocks);
     g.q_pad = l.q_pad;
     g.k_steps = static_cast<uint32_t>((a->dim + 15) / 16);
     g.n_pv = 16 * g.k_steps;
@@ -307,6 +312,12 @@ int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* w
                         : (bf16 ? go_q(tc_dq_kernel<128, true>, TcDq<128>::kBytes)
                                 : go_q(tc_dq_kernel<128, false>, TcDq<128>::kBytes)))
         return rc;
+    if (l.dq > 1) {
+        const int64_t slip_blocks = ceil_div(stats, kThreads);
+        if (int rc = simple_launch_check(slip_blocks, "tc_slips_kernel")) return rc;
+        tc_slips_kernel<<<static_cast<unsigned>(slip_blocks), kThreads, 0, st>>>(g);
+        if (int rc = rdvb_host::launched("tc_slips_kernel")) return rc;
+    }
     g.a.splits = l.dkv;
     g.a.split_len = l.dkv_len;
     const int64_t blocks = ceil_div(a->kv_len, kTcTile) * a->kv_heads * a->batch * l.dkv;
@@ -320,10 +331,6 @@ int launch_tc_backward(const rdvb_attention* a, const Plan& l, Params p, void* w
     return narrow ? (bf16 ? go(tc_dkv_kernel<64, true>, TcDkv<64>::kBytes) : go(tc_dkv_kernel<64, false>, TcDkv<64>::kBytes))
                   : (bf16 ? go(tc_dkv_kernel<128, true>, TcDkv<128>::kBytes)
                           : go(tc_dkv_kernel<128, false>, TcDkv<128>::kBytes));
-}
-
-int simple_launch_check(int64_t blocks, const char* what) {
-    return blocks > 0x7fffffffLL ? fail(RDVB_ERR_UNSUPPORTED, "%s: too many blocks", what) : RDVB_OK;
 }
 
 }  // namespace

@@ -38,6 +38,7 @@ struct GradParams {
     float* neg_lse;    // [batch, heads, q_pad]: -lse log2 e; -inf past q_len
     float* neg_delta;  // [batch, heads, q_pad]: -rowsum(dO O); 0 past q_len
     float2* norms;     // [kPrepBlocks]: largest |dO|^2 and |V|^2 of a row (float16)
+    float* slips;      // [splits of dQ, batch, heads, q_pad]: a split's sum of dS; splits > 1
     int64_t q_pad;     // q_len rounded up to whole tiles
     uint32_t k_steps, n_pv;
     int guarded;
@@ -209,9 +210,10 @@ __device__ __forceinline__ void store_columns(const Params& a, void* out, float*
 //
 // delta = rowsum(dO O) comes from the rounded O, which shows where few keys
 // matter: dP - delta is then a small difference (of one key: 0). Its exact
-// value is sum P dP. Where a row's keys are one tile, dS is made with that;
+// value is sum P dP. Where a sample's keys are one tile, dS is made with that;
 // where they are several, the sum of dS, which should be 0, is what delta was
-// off by, and the kernel of dK and dV after this one gets delta with it.
+// off by, and the kernel of dK and dV after this one gets delta with it (where
+// the keys are split, from tc_slips_kernel, which adds the splits' sums up).
 template <int DP>
 struct TcDq {
     static constexpr int kAtoms = DP / 64, kKStages = 3, kVStages = 2, kItems = DP == 64 ? 2 : 1;
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         };
         for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const TcItem t = tc_item<1>(a, id);
-            const bool one = t.tiles == 1 && a.splits == 1;
+            const bool one = t.tiles == 1 && length_of(a, t.b) <= kTcTile;
             float slip0 = 0.0f, slip1 = 0.0f;  // sum of dS
             const int64_t q = t.q0 + (warp & 3) * 32 + lane;
             const int64_t stat = (static_cast<int64_t>(t.b) * a.heads + t.h) * p.q_pad + q;
@@ -526,13 +528,17 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_full + 8 * (n & 1));
             }
-            if (t.tiles > 0 && ok && a.splits == 1) {
+            if (t.tiles > 0 && ok) {
                 if (!one) {
                     slip0 += slip1;
                     ok = row_sum(slip0);
-                    neg_delta -= slip0 * to_p;
                 }
-                if (ok && half == 0 && any && q < a.q_len) p.neg_delta[stat] = neg_delta;
+                if (ok && half == 0) {
+                    if (!one && a.splits > 1)
+                        p.slips[t.split * (static_cast<int64_t>(a.batch) * a.heads * p.q_pad) + stat] = slip0 * to_p;
+                    else if (any && q < a.q_len)
+                        p.neg_delta[stat] = one ? neg_delta : neg_delta - slip0 * to_p;
+                }
             }
             const uint32_t slot = m % F::kItems;
             if (t.tiles > 0 && ok)
@@ -567,6 +573,20 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         tmem_relinquish();
         tmem_dealloc(tmem, 512);
     }
+}
+
+// delta of rows whose keys are several tiles in several splits: the splits'
+// sums of dS in order, a thread a row. Splits past a sample's length have none.
+__global__ void __launch_bounds__(kThreads) tc_slips_kernel(const GradParams p) {
+    const Params& a = p.a;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * p.q_pad;
+    const int64_t row = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
+    if (row >= rows) return;
+    const int64_t len = length_of(a, static_cast<int>(row / p.q_pad / a.heads));
+    if (len <= kTcTile) return;
+    float sum = 0.0f;
+    for (int64_t s = 0; s * a.split_len < len; ++s) sum += p.slips[s * rows + row];
+    p.neg_delta[row] -= sum;
 }
 
 // ------------------------------------------------------------------- dK, dV

@@ -409,6 +409,69 @@ def test_attention_few_keys_gradients(rdv, cuda_device, dtype, lk, d):
         assert worst <= 1.0, (name, worst)
 
 
+def own_gradients(q, k, v, dout, keep, scale):
+    """Definition in 64 bits of dS, and what dq and dk sum of its absolute values."""
+    b, _, h, _ = q.shape
+    g = h // k.shape[2]
+    zero = torch.zeros((), dtype=torch.float64, device=q.device)
+    qd, do = q.double().permute(0, 2, 1, 3), dout.double().permute(0, 2, 1, 3)
+    kd, vd = (torch.where(keep[:, :, None, None], t.double(), zero).permute(0, 2, 1, 3).repeat_interleave(g, 1)
+              for t in (k, v))
+    s = torch.where(keep[:, None, None], qd @ kd.transpose(-1, -2) * scale, -math.inf)
+    p = torch.softmax(s, -1)
+    ds = (p * (do @ vd.transpose(-1, -2) - (do * (p @ vd)).sum(-1, keepdim=True)) * scale).abs()
+    own_k = (ds.transpose(-1, -2) @ qd.abs()).reshape(b, -1, g, *kd.shape[2:]).sum(2)
+    return (ds @ kd.abs()).permute(0, 2, 1, 3), own_k.permute(0, 2, 1, 3)
+
+
+def near_own(got, exact, dtype, own):
+    """got within dS's own rounding, u |dS|, and float32's of what it is the difference of."""
+    u = U[dtype]
+    bound = u * exact[0].abs() + u * own + 64 * 2.0 ** -24 * exact[1] + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    worst = ((got.double() - exact[0]).abs() / bound.clamp(min=1e-300)).max().item()
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("length", [1, 2, 5, 128])
+@pytest.mark.parametrize("d", [40, 64, 128])
+def test_attention_few_keys_of_long_padding(rdv, cuda_device, dtype, length, d):
+    """Few states, padded to many: the long axis is split, and the gradients keep
+    their digits as where it is not."""
+    q, k, v, dout = inputs(length + d, 2, 150, 1000, 4, 2, d, dtype)
+    lengths = [length, (length + 1) // 2]
+    keep = keep_of(k, lengths, None)
+    exact, _ = attend64(q, k, v, keep, d ** -0.5, dout)
+    out, lse = rdv.cross_attention_forward(q, k, v, lengths=lengths)
+    dq, dk, dv = rdv.cross_attention_backward(dout, q, k, v, out, lse, lengths=lengths)
+    own_q, own_k = own_gradients(q, k, v, dout, keep, d ** -0.5)
+    near_own(dq, exact["dq"], dtype, own_q)
+    near_own(dk, exact["dk"], dtype, own_k)
+    near(dv, exact["dv"][0], dtype, exact["dv"][1])
+
+
+@pytest.mark.parametrize("lq", [150, 5000])
+@pytest.mark.parametrize("d,dtype", [(40, torch.float16), (40, torch.bfloat16), (64, torch.float16),
+                                     (64, torch.bfloat16), (128, torch.bfloat16)])
+def test_attention_one_key_of_many_matters(rdv, cuda_device, dtype, lq, d):
+    """Each position all but picks one of 1000 states: dP - delta is a small
+    difference there, and dK keeps its digits whether dQ's long axis is split (few
+    positions) or not. Scores stay below 32, near()'s room for their rounding. Not
+    float16 at 128 dimensions: there the states that are not picked have
+    probabilities near 1e-9, and dS falls below the smallest step that it is held
+    with, 2^-24 of 2^-E, which near_own() does not count."""
+    q, k, v, dout = inputs(d, 2, lq, 1000, 4, 2, d, dtype)
+    pick = torch.randint(0, 1000, (2, lq), generator=gen(d + 1), device=cuda_device)
+    picked = torch.stack([k[i, pick[i]] for i in range(2)]).repeat_interleave(2, 2)
+    q = (picked.float() * 2).to(dtype)
+    lengths = [1000, 700]
+    keep = keep_of(k, lengths, None)
+    exact, _ = attend64(q, k, v, keep, d ** -0.5, dout)
+    out, lse = rdv.cross_attention_forward(q, k, v, lengths=lengths)
+    _, dk, _ = rdv.cross_attention_backward(dout, q, k, v, out, lse, lengths=lengths)
+    near_own(dk, exact["dk"], dtype, own_gradients(q, k, v, dout, keep, d ** -0.5)[1])
+
+
 def test_attention_strides_and_streams(rdv, cuda_device):
     g = gen(21)
     kv = randn(g, 2, 150, 2, 4, 64, dtype=torch.bfloat16)
