@@ -185,6 +185,20 @@ def _states(name, t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
+def _key_lengths(lengths, b, lk):
+    """lengths as the kernels take them: int32, dense. They clamp to [0, lk]
+    themselves; here only types whose values could wrap are clamped."""
+    if not (tuple(lengths.shape) == (b,) and not lengths.is_floating_point() and not lengths.is_complex()
+            and lengths.dtype != torch.bool):
+        raise ValueError(f"lengths must be whole numbers [{b}]")
+    if lengths.dtype in (torch.int64, torch.uint32, torch.uint64):
+        wide = lengths.to(torch.int64)
+        if lengths.dtype == torch.uint64:  # 2**63 and more
+            wide = wide.masked_fill(wide < 0, lk)
+        lengths = wide.clamp(0, lk)
+    return lengths.to(torch.int32).contiguous()
+
+
 def _describe(q, k, v, lengths, mask, scale):
     """The rdvb_attention of a call, as bytes, and the tensors that it points into."""
     q, k, v = _states("q", q), _states("k", k), _states("v", v)
@@ -199,12 +213,7 @@ def _describe(q, k, v, lengths, mask, scale):
     if not (kv_heads > 0 and heads > 0 and heads % kv_heads == 0):
         raise ValueError(f"k's heads ({kv_heads}) must divide q's ({heads})")
     if lengths is not None:
-        lengths = _tensor(lengths)
-        if not (tuple(lengths.shape) == (b,) and not lengths.is_floating_point() and lengths.dtype != torch.bool):
-            raise ValueError(f"lengths must be whole numbers [{b}]")
-        if lengths.dtype != torch.int32:
-            lengths = lengths.clamp(0, lk).to(torch.int32)
-        lengths = lengths.contiguous()
+        lengths = _key_lengths(_tensor(lengths), b, lk)
     if mask is not None:
         mask = _tensor(mask)
         if not (tuple(mask.shape) == (b, lk) and mask.dtype == torch.bool):

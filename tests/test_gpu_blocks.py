@@ -496,6 +496,14 @@ def test_attention_strides_and_streams(rdv, cuda_device):
     assert torch.equal(other, dense)
 
 
+def test_attention_lengths_of_narrow_types(rdv, cuda_device):
+    q, k, v, _ = inputs(17, 3, 20, 300, 2, 1, 64, torch.bfloat16)
+    values = [0, 7, 120]
+    expect = rdv.cross_attention(q, k, v, lengths=torch.tensor(values, dtype=torch.int32, device=cuda_device))
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int64, torch.uint16, torch.uint32, torch.uint64):
+        assert torch.equal(rdv.cross_attention(q, k, v, lengths=torch.tensor(values, dtype=dtype, device=cuda_device)), expect)
+
+
 def test_attention_empty(rdv, cuda_device):
     for b, lq, lk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
         q, k, v, dout = inputs(1, b, lq, lk, 2, 1, 64, torch.float16)
