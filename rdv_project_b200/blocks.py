@@ -19,7 +19,8 @@ The reference has none of them.
 Elements are float32, float16 or bfloat16; results have their input's type,
 sums and statistics are float32. The three main functions are
 differentiable: where gradients are enabled and an input requires one, they
-record themselves for torch's autograd. Calls are asynchronous on the
+record themselves for torch's autograd, in reverse mode; inputs with a
+forward-mode tangent are refused. Calls are asynchronous on the
 current stream, with workspaces from torch's allocator.
 """
 from __future__ import annotations
@@ -27,6 +28,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .core import RDVObject, _timed, as_device_tensor, current_device, stream_handle, wrap
@@ -57,6 +59,12 @@ def _ptr(t):
 
 
 def _wants_grad(*tensors) -> bool:
+    """Whether a call is to be recorded for its gradients. Forward-mode
+    derivatives, which the kernels do not carry along, are refused."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the image block's operators have no forward-mode derivative")
     if not torch.is_grad_enabled():
         return False
     for t in tensors:

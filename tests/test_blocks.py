@@ -1,6 +1,7 @@
 """CPU tests of the conditioned image block's host side (blocks.py)."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 WHOLE = [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16, torch.uint32, torch.uint64]
 
@@ -27,3 +28,19 @@ def test_lengths_refusals():
                 torch.zeros(3, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int64), torch.tensor(3)):
         with pytest.raises(ValueError):
             _key_lengths(bad, 2, 9)
+
+
+def test_forward_mode_inputs_are_refused():
+    """A tangent is not dropped in silence, with gradients enabled or not."""
+    import rdv_project_b200 as rdv
+
+    x, w, q = torch.ones(2, 3, 8), torch.ones(8), torch.ones(1, 2, 2, 8)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: rdv.group_norm(dual(x), 2), lambda: rdv.group_norm(x, 2, dual(w)),
+                     lambda: rdv.group_norm(x, 2, w, dual(w)), lambda: rdv.cross_attention(dual(q), q, q),
+                     lambda: rdv.cross_attention(q, dual(q), q), lambda: rdv.cross_attention(q, q, dual(q)),
+                     lambda: rdv.dropout(dual(x), 0.1, 0), lambda: rdv.dropout(x, 0.1, 0, residual=dual(x))):
+            for enabled in (True, False):
+                with torch.set_grad_enabled(enabled), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
