@@ -61,6 +61,7 @@ def _ptr(t):
 def _wants_grad(*tensors) -> bool:
     """Whether a call is to be recorded for its gradients. Forward-mode
     derivatives, which the kernels do not carry along, are refused."""
+    tensors = [t._tensor if isinstance(t, RDVObject) else t for t in tensors]
     if forward_ad._current_level >= 0:
         for t in tensors:
             if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:

@@ -44,3 +44,16 @@ def test_forward_mode_inputs_are_refused():
             for enabled in (True, False):
                 with torch.set_grad_enabled(enabled), pytest.raises(NotImplementedError, match="forward-mode"):
                     call()
+
+
+def test_wrapped_inputs_ask_for_gradients_like_their_tensors():
+    import rdv_project_b200 as rdv
+    from rdv_project_b200.blocks import _wants_grad
+
+    x = torch.ones(2, 8)
+    wrapped = rdv.wrap(x.clone().requires_grad_())
+    assert _wants_grad(None, wrapped) and not _wants_grad(rdv.wrap(x), None)
+    with torch.no_grad():
+        assert not _wants_grad(wrapped)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        _wants_grad(rdv.wrap(forward_ad.make_dual(x, x)))

@@ -678,6 +678,20 @@ def test_autograd_matches_explicit_gradients(rdv, cuda_device):
     assert torch.equal(x.grad, rdv.dropout_backward(dy, 0.2, 5, 6)) and torch.equal(r.grad, dy)
 
 
+def test_autograd_of_wrapped_inputs(rdv, cuda_device):
+    g = gen(42)
+    x, dy = randn(g, 2, 30, 64), randn(g, 2, 30, 64)
+    for call, shape in ((lambda t: rdv.group_norm(t, 8, activation="silu"), (2, 30, 64)),
+                        (lambda t: rdv.dropout(t, 0.2, 5), (2, 30, 64)),
+                        (lambda t: rdv.cross_attention(t, t, t), (2, 30, 1, 64))):
+        grads = []
+        for wrap in (rdv.wrap, lambda t: t):
+            t = x.reshape(shape).clone().requires_grad_()
+            call(wrap(t)).backward(dy.reshape(shape))
+            grads.append(t.grad)
+        assert torch.equal(*grads)
+
+
 def test_tensor_operations(rdv, cuda_device):
     g = gen(50)
     x, w, b = randn(g, 16 * 16, 32), 1 + 0.1 * randn(g, 32), randn(g, 32)
