@@ -128,7 +128,7 @@ def group_norm_forward(x, groups: int, weight=None, bias=None, eps: float = 1e-5
 
 
 def _as_param(grad, param):
-    kind = getattr(param, "dtype", torch.float32)
+    kind = getattr(param._tensor if isinstance(param, RDVObject) else param, "dtype", torch.float32)
     return grad if grad is None or kind not in _DTYPES else grad.to(kind)
 
 

@@ -692,6 +692,15 @@ def test_autograd_of_wrapped_inputs(rdv, cuda_device):
         assert torch.equal(*grads)
 
 
+def test_gradients_have_their_parameters_type(rdv, cuda_device):
+    g = gen(43)
+    x, w = randn(g, 2, 30, 64), randn(g, 64).half()
+    y, stats = rdv.group_norm_forward(x, 8, w, w)
+    for param in (w, rdv.wrap(w)):
+        _, dw, db = rdv.group_norm_backward(y, x, stats, 8, param, param)
+        assert dw.dtype == db.dtype == torch.float16
+
+
 def test_tensor_operations(rdv, cuda_device):
     g = gen(50)
     x, w, b = randn(g, 16 * 16, 32), 1 + 0.1 * randn(g, 32), randn(g, 32)
