@@ -61,17 +61,16 @@ def _ptr(t):
 def _wants_grad(*tensors) -> bool:
     """Whether a call is to be recorded for its gradients. Forward-mode
     derivatives, which the kernels do not carry along, are refused."""
-    tensors = [t._tensor if isinstance(t, RDVObject) else t for t in tensors]
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("the image block's operators have no forward-mode derivative")
-    if not torch.is_grad_enabled():
-        return False
+    tangents = forward_ad._current_level >= 0
+    wants = False
     for t in tensors:
-        if isinstance(t, torch.Tensor) and t.requires_grad:
-            return True
-    return False
+        if isinstance(t, RDVObject):
+            t = t._tensor
+        if tangents and isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the image block's operators have no forward-mode derivative")
+        if getattr(t, "requires_grad", False):
+            wants = True
+    return wants and torch.is_grad_enabled()
 
 
 # ---------------------------------------------------------------- group norm
