@@ -17,7 +17,10 @@ The reference has none of them.
   ``TensorOperation`` s (fp32 ``[rows, channels]``, one sample).
 
 Elements are float32, float16 or bfloat16; results have their input's type,
-sums and statistics are float32. The three main functions are
+sums and statistics are float32. 16-bit attention on the tensor cores rounds
+probabilities and score gradients to that type before the products that take
+them (float32 inputs, and 16-bit ones that the tensor cores do not take, keep
+them in float32). The three main functions are
 differentiable: where gradients are enabled and an input requires one, they
 record themselves for torch's autograd, in reverse mode; inputs with a
 forward-mode tangent are refused. Calls are asynchronous on the
@@ -196,12 +199,15 @@ def _states(name, t):
 def _key_lengths(lengths, b, lk):
     """lengths as the kernels take them: int32, dense. They clamp to [0, lk]
     themselves; here only types whose values could wrap are clamped."""
-    if not (tuple(lengths.shape) == (b,) and not lengths.is_floating_point() and not lengths.is_complex()
-            and lengths.dtype != torch.bool):
+    kind = lengths.dtype
+    if not (lengths.shape == (b,) and (kind == torch.int32 or not (
+            kind.is_floating_point or kind.is_complex or kind == torch.bool))):
         raise ValueError(f"lengths must be whole numbers [{b}]")
-    if lengths.dtype in (torch.int64, torch.uint32, torch.uint64):
+    if kind == torch.int32:
+        return lengths.contiguous()
+    if kind in (torch.int64, torch.uint32, torch.uint64):
         wide = lengths.to(torch.int64)
-        if lengths.dtype == torch.uint64:  # 2**63 and more
+        if kind == torch.uint64:  # 2**63 and more
             wide = wide.masked_fill(wide < 0, lk)
         lengths = wide.clamp(0, lk)
     return lengths.to(torch.int32).contiguous()
