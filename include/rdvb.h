@@ -581,8 +581,11 @@ int rdvb_group_norm_backward(const void* dy, const void* x, const float* stats, 
  * -inf, no gradient). What lies at a key that is not allowed is not used,
  * NaN and infinities included. Strides in elements of (sample, position,
  * head); the last dimension is dense. 16-bit inputs whose dim and strides are
- * multiples of 8 and pointers 16-byte aligned, dim <= 128 and scale >= 0 run
- * on the tensor cores, others in float32 on CUDA cores. */
+ * multiples of 8 and pointers 16-byte aligned, dim <= 128 and scale > 0 run
+ * on the tensor cores, where probabilities and score gradients are rounded to
+ * the inputs' type before the products that take them; others in float32 on
+ * CUDA cores, as do up to eight rows (positions times query heads) a key head
+ * in the forward pass. */
 typedef struct rdvb_attention {
     const void* q;
     const void* k;

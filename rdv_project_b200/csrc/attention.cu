@@ -100,8 +100,9 @@ int tile_of(const rdvb_attention* a, bool tc) { return tc ? kTcTile : a->dim > 1
 // Parts that the long axis is split into: those that make the launch
 // shortest. `blocks` blocks of `steps` loop steps run `slots` at a time, a
 // step takes step_us; parts are written and read once more by a join
-// (part_bytes each, at 3 TB/s with their launches' ends, and 4 us of launch). At least two steps a
-// part, at most 32 parts.
+// (part_bytes each, at 3 TB/s with their launches' ends, and 4 us of launch;
+// the sum of dQ's row sums, 2.4 us, is not counted). At least two steps a part,
+// at most 32 parts.
 int splits_for(int64_t blocks, int64_t steps, int64_t slots, double step_us, double part_bytes) {
     int best = 1;
     double least = 0.0;
@@ -131,8 +132,8 @@ Plan plan(const rdvb_attention* a) {
     const int64_t q_tiles = ceil_div(a->q_len, tile), k_tiles = ceil_div(a->kv_len, tile);
     const int64_t rows = static_cast<int64_t>(a->batch) * a->q_len * a->heads;
     const int64_t kv_rows = static_cast<int64_t>(a->batch) * a->kv_len * a->kv_heads;
-    // The tensor-core kernels hold one block a processor (the forward one takes two query tiles), the CUDA-core ones
-    // two. Microseconds a step, measured: 128 keys against 256 queries, 128 x 128 for dQ and for dK and dV; 64 x 64.
+    // The tensor-core kernels hold one block a processor (the forward one takes two query tiles). The CUDA-core ones
+    // are counted as two; above 64 dimensions shared memory holds one (129 to 256 forward: two). Microseconds a step, measured: 128 keys against 256 queries, 128 x 128 for dQ and for dK and dV; 64 x 64.
     const int64_t slots = p.tc ? 148 : 296;
     const bool narrow = a->dim <= 64;
     const double row_bytes = static_cast<double>(a->dim) * 4;
@@ -141,7 +142,8 @@ Plan plan(const rdvb_attention* a) {
     p.forward_len = ceil_div(k_tiles, p.forward) * tile;
     p.few = few_rows(a);
     if (p.few) {
-        // three blocks a processor stream the keys, 64 or more each
+        // three blocks a processor stream the keys, 64 or more each (223 pairs of a sample and a key head, or more:
+        // a block each)
         const int64_t heads = static_cast<int64_t>(a->batch) * a->kv_heads;
         const int64_t most = std::min<int64_t>(ceil_div(a->kv_len, 64), kMaxSplits);
         const int64_t want = std::max<int64_t>(1, std::min(most, 3 * 148 / std::max<int64_t>(heads, 1)));

@@ -13,18 +13,21 @@
 // item's first products and loads run beside this one's last rows. Warps 0-3
 // and 4-7: softmax of a tile each. Warp 8: loads. Warps 9 and 11: products of
 // a tile each up to 64 dimensions (one thread issues a product in 60 to 110
-// cycles; two took 1000 to 869 us off the first case below), at 128 warp 9 for both
+// cycles; with two, the first case below went from 1000 to 869 us, before masks were
+// read a tile ahead, which costs it 41), at 128 warp 9 for both
 // (two: 1169 to 1620 us, their products delaying each other's). Warp 10: zeroes the
 // rows of V whose keys are not allowed (their P is 0, but 0 times NaN is not).
 //
 // S, the row sums and O are float32; P is rounded to the inputs' type, as the
-// tensor cores take it. O is rescaled only when a row's maximum has grown by
+// tensor cores take it (P in float32 as two 16-bit parts would take half as many
+// products again): where the rounding of O alone leaves 2.1e-4 of the result in
+// float16, it is 2.5e-4 with it. O is rescaled only when a row's maximum has grown by
 // more than 2^8 since the last time: P stays below 2^8, well inside both types.
 // The scale is above 0, so that the largest score is the scaled largest
 // product and a score of -inf stays one.
 //
-// Measured (bfloat16): 16384 x 4096, 2 samples of 16 heads of 64, 912 us, 603
-// TFLOP/s; 16384 x 4099, 16 heads of 128 over 4, 1180 us, 935 TFLOP/s. Bound: the
+// Measured (bfloat16): 16384 x 4096, 2 samples of 16 heads of 64, 910 us, 604
+// TFLOP/s; 16384 x 4099, 16 heads of 128 over 4, 1176 us, 935 TFLOP/s. Bound: the
 // chain of a tile -- scores, about 1,100 cycles of exponentials, the product
 // that takes them -- of which two tiles overlap; the tensor pipe is 23 and 36 %
 // busy, the exponential unit 42 %.
@@ -51,7 +54,7 @@ struct TcParams {
     uint32_t* status;
     uint32_t k_steps;  // ceil(dim / 16)
     uint32_t n_pv;     // dim rounded up to 16
-    int guarded;       // lengths or a mask: warp 6 takes part
+    int guarded;       // lengths or a mask: warp 10 takes part
 };
 
 // The tensor map of q, k or v, and whether its head and sample axes are walked
@@ -157,18 +160,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -19,7 +19,8 @@ struct Plan {
 };
 
 // Slabs of a sample: four blocks a processor over the batch, so that one round
-// of blocks does it, but at least 16 rows each.
+// of blocks does it, but at least 16 rows each and at most kMaxSlabs a sample
+// (of up to four samples, fewer blocks than that).
 Plan plan(int64_t n, int64_t rows, int c, int groups, int backward) {
     Plan a;
     const int64_t want = std::max<int64_t>(1, 592 / std::max<int64_t>(n, 1));
