@@ -22,7 +22,9 @@
 // tensor cores take it (P in float32 as two 16-bit parts would take half as many
 // products again): where the rounding of O alone leaves 2.1e-4 of the result in
 // float16, it is 2.5e-4 with it. O is rescaled only when a row's maximum has grown by
-// more than 2^8 since the last time: P stays below 2^8, well inside both types.
+// more than 2^8 since the last time: P stays below 2^8. float16 has few exponents:
+// it holds P times 2^7, so that a probability keeps its digits down to 2^-21 of
+// its row's largest (and is 0 below 2^-32).
 // The scale is above 0, so that the largest score is the scaled largest
 // product and a score of -inf stays one.
 //
@@ -521,7 +523,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t col_s = row_base + F::kColS + 128 * w, col_o = row_base + F::kColO + DP * w,
                        col_p = row_base + F::kColP + F::kStepP * w;
         const float c = a.scale * kLog2e;
-        uint32_t n = 0;  // key tiles of this query tile so far
+        constexpr float kHeld = kBf16 ? 0.0f : 7.0f;  // P, its sum and O are held times 2^kHeld
+        uint32_t n = 0;                               // key tiles of this query tile so far
         bool ok = true;
         for (uint32_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const TcItem t = tc_item<2>(a, id);
@@ -594,7 +597,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                 }
-                const float minus = top == -INFINITY ? 0.0f : -top;
+                const float minus = top == -INFINITY ? 0.0f : kHeld - top;
                 float sum[4] = {};
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -662,11 +665,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (mine) {
                 if (a.splits > 1) {
-                    a.part_stat[2 * (t.split * rows + row)] = top;
+                    a.part_stat[2 * (t.split * rows + row)] = top - kHeld;
                     a.part_stat[2 * (t.split * rows + row) + 1] = any ? total : -1.0f;
                 } else if (a.lse) {
                     a.lse[(static_cast<int64_t>(t.b) * a.heads + t.h) * a.q_len + q] =
-                        any ? (top + log2f(total)) * kLn2 : -INFINITY;
+                        any ? (top - kHeld + log2f(total)) * kLn2 : -INFINITY;
                 }
             }
         }

@@ -367,6 +367,29 @@ def test_attention_extreme_scores(rdv, cuda_device, dtype):
     assert torch.isnan(out[0, :, 0, 3]).all() and torch.isfinite(out[0, :, 1]).all() and torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lq", [1, 150, 5000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_many_small_probabilities(rdv, cuda_device, dtype, lq, d):
+    """One state takes nearly all of the softmax and has no value, so that the
+    result is the others', whose probabilities are equal and 2^-12 to 2^-20.5 of
+    the largest: what rounding does to one it does to all. A probability in 16 bits
+    keeps its digits there, u of it, and is inside near()'s two."""
+    g = gen(d + lq)
+    lk = 1500
+    q, k, v = (torch.zeros(2, n, h, d, dtype=dtype, device=cuda_device) for n, h in ((lq, 4), (lk, 2), (lk, 2)))
+    q[..., 0] = 1
+    v[:] = 0.5 + randn(g, *v.shape).abs()
+    v[:, 700] = 0
+    for low in (12.0, 16.5, 20.5):
+        k[:, 700, :, 0] = low * math.log(2)
+        result, lse64 = attend64(q, k, v, keep_of(k, None, None), 1.0)
+        exact, mass = result["out"]
+        out, lse = rdv.cross_attention_forward(q, k, v, scale=1.0)
+        near(out, exact, dtype, mass)
+        assert ((lse.double() - lse64).abs() <= 64 * 2.0 ** -24 * (1 + lse64.abs())).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_attention_small_gradients(rdv, cuda_device, dtype):
     """Gradients far below and above 1 (a scaled loss) keep their digits."""
