@@ -745,6 +745,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
             for (int i = 0; i < items; ++i) {
                 const uint32_t s = i % F::kStages, half = i & 1, at = s * (F::kTileBytes / 16);
                 if (!mbar_wait(p_full + 8 * half, (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull)) break;
+                // P(i) says that Q(i) has come, not that dO(i) has
+                if (!mbar_wait(do_full + 8 * s, (i / F::kStages) & 1, abort_flag, p.status, kStatusTimeoutXFull)) break;
                 tc_fence_after();
                 product_columns(tmem + F::kColDv, tmem + F::col_s(i), do_desc + at, idesc, i == 0);
                 if (!mbar_wait(ds_full + 8 * half, (i / 2) & 1, abort_flag, p.status, kStatusTimeoutAFull)) break;

@@ -519,6 +519,28 @@ def test_attention_strides_and_streams(rdv, cuda_device):
     assert torch.equal(other, dense)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 1248, 2372, 1, 1, 8), (2, 1100, 900, 4, 2, 64), (2, 1100, 900, 4, 1, 128)])
+def test_attention_repeats_beside_other_traffic(rdv, cuda_device, dtype, shape):
+    """The same bits every time while another stream keeps the memory busy, so that
+    the kernels' copies arrive late and in other orders."""
+    q, k, v, dout = inputs(sum(shape), *shape, dtype)
+    lengths = [shape[2]] * (shape[0] - 1) + [shape[2] // 3]
+    out, grads = check_attention(rdv, q, k, v, dout, torch.tensor(lengths, device=cuda_device))
+    lengths = torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    src = torch.zeros(2 ** 28, dtype=torch.uint8, device=cuda_device)
+    dst = torch.empty_like(src)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(60):
+        with torch.cuda.stream(side):
+            dst.copy_(src)
+        again, lse = rdv.cross_attention_forward(q, k, v, lengths=lengths)
+        grads_again = rdv.cross_attention_backward(dout, q, k, v, again, lse, lengths=lengths)
+        assert torch.equal(again, out) and all(torch.equal(a, e) for a, e in zip(grads_again, grads))
+    torch.cuda.current_stream().wait_stream(side)
+
+
 def test_attention_lengths_of_narrow_types(rdv, cuda_device):
     q, k, v, _ = inputs(17, 3, 20, 300, 2, 1, 64, torch.bfloat16)
     values = [0, 7, 120]
